@@ -215,6 +215,49 @@ int iso_rows_pack(int P, int F, const unsigned char* touched, const float* grad,
 int iso_rows_scatter_add(int F, int P, long long max_rows, const int* count, const int* idx, const float* rows, float* dst, int assign,
                          void* stream);
 
+/* ---- rows and gradients (types: 0 float32, 1 bfloat16, 2 float16; strides in elements between rows whose columns lie together; views may
+ * start at any element) ------------------------------------------------------------------------------------------------------------
+ * Root-mean-square norm of rows with the residual's addition:
+ *   s = x + residual (32 bits),  rstd = 1 / sqrt(mean(s^2) + eps),  y = s rstd weight
+ * residual, weight, s_out and rstd may be NULL; y and s_out are [rows, F] of x's type, each rounded once; weight is of x's type or
+ * float32 (weight_is_float).  eps > 0.  A row that holds an infinity or NaN gives NaN at those places (a NaN: in the whole row). */
+int iso_rms_norm_forward(int type, long long rows, int F, const void* x, long long x_stride, const void* residual,
+                         long long residual_stride, const void* weight, int weight_is_float, float eps, void* y, void* s_out,
+                         float* rstd /*[rows]*/, void* stream);
+/* The same with y in 8 bits: codes [rows, F] (code 1: int8, 2: e4m3), scales [rows, F / group]; y is about code * scale.  Per group of
+ * `group` columns (F, or 32 / 64 / 128 dividing F): top = max |s weight|, code = s weight Q / top to the nearest, ties to even,
+ * scale = top rstd / Q, Q = 127 (int8) or 448 (e4m3).  Groups below 2^-116 are zeros; a group with an infinity or NaN has scale NaN. */
+int iso_rms_norm_quant(int type, int code, long long rows, int F, int group, const void* x, long long x_stride, const void* residual,
+                       long long residual_stride, const void* weight, int weight_is_float, float eps, void* codes, float* scales,
+                       void* s_out, void* stream);
+/* Backward, from s (the forward's s_out, or x without a residual) and rstd:  h = s rstd,
+ *   ds = rstd (gy weight - h mean(gy weight h)) + gs      the gradient of x and of the residual
+ *   dw = sum over rows of gy h                            in weight's type; summed in 32 bits in an order that rows and F alone fix
+ * gs (the gradient that reaches s_out) may be NULL; ds or dw may be NULL.  scratch: iso_rms_norm_scratch_bytes, needed with dw. */
+size_t iso_rms_norm_scratch_bytes(int type, long long rows, int F);
+int iso_rms_norm_backward(int type, long long rows, int F, const void* s, long long s_stride, const void* weight, int weight_is_float,
+                          const float* rstd, const void* gy, long long gy_stride, const void* gs, long long gs_stride, void* ds,
+                          void* dw, void* scratch, size_t scratch_bytes, void* stream);
+
+/* A table of P rows in 8 bits: codes [P, F], scales [P, F / group], rounded per group as by iso_rms_norm_quant without a norm
+ * (scale = top / Q).  Rows are written to [first, first + n) (index NULL) or to index[i] (int64 or int32): of equal indices the last one is
+ * kept, an index outside [0, P) writes nothing.  Beyond ISO_ROWS8_SCAN indices `owner` is needed: [P] ints, all -1 before the first
+ * call; every call leaves them all -1 again. */
+#define ISO_ROWS8_SCAN 256
+int iso_rows8_write(int type, int code, long long n, int F, int group, long long P, const void* rows, long long row_stride, long long first,
+                    const void* index, int index_is_int64, int* owner, void* codes, float* scales, void* stream);
+/* out[i, :] = the values of row first + i or index[i] (an index outside [0, P): zeros), divided by (|row|_2 + eps) if normalize. */
+int iso_rows8_read(int type, int code, long long n, int F, int group, long long P, const void* codes, const float* scales, long long first,
+                   const void* index, int index_is_int64, int normalize, float eps, void* out, void* stream);
+
+/* The norm of all elements of `count` tensors together - norm_type 2, 1, or 0 for the largest magnitude - and, with clip, their scaling in
+ * place:  out[0] = norm,  out[1] = coef = min(1, max_norm / (norm + 1e-6)),  tensor *= coef (left alone where coef is 1).
+ * tensors / sizes / types are HOST arrays; a size may be 0; with clip no two tensors may share memory.  Sums are held in 64 bits, in an order
+ * that the sizes alone fix.  scratch: iso_grad_norm_scratch_bytes of device memory. */
+size_t iso_grad_norm_scratch_bytes(int count, const long long* sizes);
+int iso_grad_norm(int count, void* const* tensors, const long long* sizes, const int* types, int norm_type, float max_norm, int clip,
+                  float* out /*[2]*/, void* scratch, size_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -110,6 +110,19 @@ SIGNATURES = {
     "iso_flag_wait": (c_int, [c_int, _P, c_int, c_uint, _P, c_int, _P]),
     "iso_rows_pack": (c_int, [c_int, c_int, _P, _P, _P, _P, _P, _P]),
     "iso_rows_scatter_add": (c_int, [c_int, c_int, ctypes.c_longlong, _P, _P, _P, _P, c_int, _P]),
+    "iso_rms_norm_forward": (c_int, [c_int, ctypes.c_longlong, c_int, _P, ctypes.c_longlong, _P, ctypes.c_longlong, _P, c_int, c_float, _P,
+                                     _P, _P, _P]),
+    "iso_rms_norm_quant": (c_int, [c_int, c_int, ctypes.c_longlong, c_int, c_int, _P, ctypes.c_longlong, _P, ctypes.c_longlong, _P, c_int,
+                                   c_float, _P, _P, _P, _P]),
+    "iso_rms_norm_scratch_bytes": (c_size_t, [c_int, ctypes.c_longlong, c_int]),
+    "iso_rms_norm_backward": (c_int, [c_int, ctypes.c_longlong, c_int, _P, ctypes.c_longlong, _P, c_int, _P, _P, ctypes.c_longlong, _P,
+                                      ctypes.c_longlong, _P, _P, _P, c_size_t, _P]),
+    "iso_rows8_write": (c_int, [c_int, c_int, ctypes.c_longlong, c_int, c_int, ctypes.c_longlong, _P, ctypes.c_longlong, ctypes.c_longlong,
+                                _P, c_int, _P, _P, _P, _P]),
+    "iso_rows8_read": (c_int, [c_int, c_int, ctypes.c_longlong, c_int, c_int, ctypes.c_longlong, _P, _P, ctypes.c_longlong, _P, c_int, c_int,
+                               c_float, _P, _P]),
+    "iso_grad_norm_scratch_bytes": (c_size_t, [c_int, _P]),
+    "iso_grad_norm": (c_int, [c_int, _P, _P, _P, c_int, c_float, c_int, _P, _P, c_size_t, _P]),
     "iso_rownorm2": (c_int, [ctypes.c_longlong, c_int, c_float, c_float, c_int, _P, _P, _P, _P, _P, _P]),
 }
 
@@ -117,7 +130,7 @@ SIGNATURES = {
 def build(force: bool = False) -> str:
     """Compile the HIP library for gfx950 with hipcc (cross-compiles without a GPU)."""
     src_dir = os.path.join(_HERE, "csrc")
-    args = ["make", "-C", src_dir, "-s", "-j", str(min(5, os.cpu_count() or 1))]
+    args = ["make", "-C", src_dir, "-s", "-j", str(min(6, os.cpu_count() or 1))]
     if force:
         args.append("-B")
     subprocess.check_call(args)

@@ -12,6 +12,7 @@ import torch
 
 from . import _hot
 from ._lib import check, lib
+from .rows import QuantizedRows
 
 
 def _p(t):
@@ -341,7 +342,10 @@ def _slot_consumed(slot: torch.Tensor, P: int, n_rows: int):
 
 
 def gather_rows(table: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
-    """``table[idx]`` for a ``[P,F]`` table and int64 row indices (train_semantic.py:183-190)."""
+    """``table[idx]`` for a ``[P,F]`` table and int64 row indices (train_semantic.py:183-190); from a ``rows.QuantizedRows`` table
+    the rows' values in float32 (no gradient)."""
+    if isinstance(table, QuantizedRows):
+        return table.read(idx)
     return _GatherRows.apply(table, idx)
 
 

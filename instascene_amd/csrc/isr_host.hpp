@@ -1,12 +1,13 @@
 // Host-side glue shared by the translation units of libinstascene_hip.so.
 //
-// The library is built from five translation units (Makefile, `make -j5`), each = the kernels of one stage plus the C-ABI
+// The library is built from six translation units (Makefile, `make -j6`), each = the kernels of one stage plus the C-ABI
 // entry points that launch them:
 //   isr_api_forward.hip       K1 preprocess, the EXACT forward blend (K8), state read-back, profiling, error text
 //   isr_api_binning.hip       K2-K7: scans, scatter into tile buckets, per-bucket sorts
 //   isr_api_forward_fast.hip  the FAST forward blend (K8, k_render_fwd_fast)
 //   isr_api_backward.hip      K9-K11: the blend backward kernels, row reductions, fused feature tail, markVisible
 //   isr_api_ops.hip           include/instascene_ops.h: k-NN, contrastive loss, render() post-processing, SSIM, optimisers
+//   isr_api_rows.hip          include/instascene_ops.h: root-mean-square norm, the 8-bit row table, the global gradient norm
 // No device code crosses a unit (no -fgpu-rdc); what the units share on the host is declared here.
 #pragma once
 #include <atomic>

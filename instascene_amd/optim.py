@@ -12,11 +12,15 @@ loss -> ``backward()`` -> ``step()``.  Arithmetic and semantics are dense ``torc
 visible still decays its moments and moves by its momentum); ``tests/test_gpu_harness.py`` pins it against torch's
 optimiser.  Row edits by the density control (clone / split / prune) are not supported here: ``RgbTrainer(densify=...)``
 keeps ``torch.optim.Adam``.
+
+Beside it, for any list of gradients: their global norm (:func:`grad_norm`) and clipping (:func:`clip_grads_`,
+:func:`clip_grad_norm_`) in one pass over all tensors each (``iso_grad_norm``, csrc/iso_gradnorm.hip).
 """
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, Optional
+import math
+from typing import Dict, Iterable, Optional, Sequence
 
 import torch
 
@@ -131,3 +135,90 @@ class GaussianAdam:
                 self.exp_avg_sq[g].copy_(st["exp_avg_sq"])
                 self.step_count = int(float(st["step"]))
         self._acts = None
+
+
+# -- the global norm of many gradients, and clipping ----------------------------------------------------------------------------
+_GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORM_TYPES = {1.0: 1, 2.0: 2, math.inf: 0}
+
+
+def _is_dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill one stretch of memory, each once (in any order of the dimensions)."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _norm_launch(what, tensors, norm_type, max_norm, clip):
+    kind = _NORM_TYPES.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"{what}: norm_type must be 1, 2 or inf, not {norm_type}")
+    dev = tensors[0].device
+    flat, back = [], []
+    for t in tensors:
+        if t.layout != torch.strided or not t.is_cuda:
+            raise RuntimeError(f"{what}: needs dense CUDA tensors (the HIP library is the only backend)")
+        if t.dtype not in _GRAD_TYPES:
+            raise TypeError(f"{what}: float32, bfloat16 or float16 gradients, not {t.dtype}")
+        if t.device != dev:
+            raise ValueError(f"{what}: all gradients must be on one device, not {dev} and {t.device}")
+        if not _is_dense(t):
+            if clip and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                raise ValueError(f"{what}: an expanded tensor cannot be clipped in place")
+            c = t.contiguous()
+            back.append((t, c))
+            t = c
+        flat.append(t)
+    n = len(flat)
+    sizes = (ctypes.c_longlong * n)(*[t.numel() for t in flat])
+    L = lib()
+    nbytes = L.iso_grad_norm_scratch_bytes(n, sizes)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    out = torch.empty(2, dtype=torch.float32, device=dev)
+    with _hot.on_device(dev):
+        check(L.iso_grad_norm(n, (ctypes.c_void_p * n)(*[t.data_ptr() for t in flat]), sizes,
+                              (ctypes.c_int * n)(*[_GRAD_TYPES[t.dtype] for t in flat]), kind, float(max_norm), int(clip), out.data_ptr(),
+                              scratch.data_ptr(), nbytes, _hot.raw_stream(dev)), "iso_grad_norm")
+    if clip:
+        torch.autograd.graph.increment_version(flat)         # the kernel wrote through raw pointers
+        for t, c in back:
+            t.copy_(c)
+    return out
+
+
+def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """The norm (2, 1 or inf) of all elements of ``tensors`` together, as a float32 scalar on their device; nothing is synchronised.
+    float32, bfloat16 and float16 may be mixed; sums are held in 64 bits.  No tensors: 0."""
+    tensors = [t.detach() for t in ([tensors] if isinstance(tensors, torch.Tensor) else tensors)]
+    if not tensors:
+        return torch.tensor(0.0)
+    return _norm_launch("grad_norm", tensors, norm_type, 0.0, False)[0]
+
+
+def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scale ``grads`` in place by ``min(1, max_norm / (norm + 1e-6))`` and return their norm before it: what
+    ``torch.nn.utils.clip_grad_norm_`` does, on a list of gradients.  The factor stays on the device; gradients that need no clipping are
+    read once and not written.  Two of them may not share memory.  ``error_if_nonfinite`` reads the norm back (a synchronisation) and
+    raises before anything is scaled."""
+    grads = [g.detach() for g in ([grads] if isinstance(grads, torch.Tensor) else grads)]
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grads_: max_norm must not be negative, is {max_norm}")
+    if not grads:
+        return torch.tensor(0.0)
+    if error_if_nonfinite:
+        norm = grad_norm(grads, norm_type)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"clip_grads_: the norm of order {norm_type} of the gradients is {float(norm)}; nothing was clipped")
+    return _norm_launch("clip_grads_", grads, norm_type, max_norm, True)[0]
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """:func:`clip_grads_` on the ``.grad`` of ``parameters`` (those that have one)."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    return clip_grads_([p.grad for p in parameters if p.grad is not None], max_norm, norm_type, error_if_nonfinite)

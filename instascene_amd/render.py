@@ -13,6 +13,7 @@ import torch
 
 from . import _hot, _lib
 from .contrastive import row_normalize
+from .rows import QuantizedRows
 from . import rasterizer as _rz
 from .rasterizer import GaussianRasterizationSettings, GaussianRasterizer
 
@@ -250,7 +251,9 @@ def render(viewpoint_camera, pc, pipe, bg_color: torch.Tensor, scaling_modifier=
 
     means2D = screenspace_points
     seg_feature = pc.get_seg_feature
-    if seg_feature is not None and norm_seg_feat:
+    if isinstance(seg_feature, QuantizedRows):              # a table kept in 8 bits: read back and normalised in one pass
+        seg_feature = seg_feature.read(norm_eps=1e-9 if norm_seg_feat else None)
+    elif seg_feature is not None and norm_seg_feat:
         seg_feature = row_normalize(seg_feature, 1e-9)      # reference :61-62
 
     # opt-in (pipe.feature_only_forward, like lazy_maps): a trainer that reads nothing but the feature map - the whole of

@@ -1,0 +1,191 @@
+"""The global gradient norm and clipping on the GPU against 64-bit sums.
+
+Sums are held in 64 bits, so the norm is one root in 64 bits and one rounding to float32: within 2 u (u = 2^-24).  The factor
+max_norm / (norm + 1e-6) adds two roundings (4 u in all), a clipped element one product (u) and one rounding to its type (half(T))."""
+import math
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from instascene_amd._lib import IsrError
+    from instascene_amd.optim import clip_grad_norm_, clip_grads_, grad_norm
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def make(sizes, seed, types=TYPES, scale=0.1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [(torch.randn(n, generator=g, device="cuda") * scale).to(types[i % len(types)]) for i, n in enumerate(sizes)]
+
+
+def exact(grads, p):
+    if p == math.inf:
+        return max([float(g.double().abs().max()) for g in grads if g.numel()], default=0.0)
+    s = sum(float(g.double().abs().pow(p).sum()) for g in grads)
+    return s ** (1.0 / p)
+
+
+LISTS = [[1], [7], [0], [0, 5, 0], [8192], [8193, 1], [1, 2, 3, 4, 5], [300, 70001, 4, 16384], [3] * 127, [5] * 128, [9] * 129, [40] * 700, [2_000_003]]
+
+
+@pytest.mark.parametrize("sizes", LISTS, ids=lambda s: f"{len(s)}x{s[0]}")
+@pytest.mark.parametrize("p", [2.0, 1.0, math.inf])
+def test_norm_and_clip(sizes, p):
+    grads = make(sizes, len(sizes))
+    want = exact(grads, p)
+    assert abs(float(grad_norm(grads, p)) - want) <= 2 * U * want
+    for factor in (0.3, 1.5, 0.0):
+        copies = [g.clone() for g in grads]
+        got = clip_grads_(copies, factor * want, p)
+        assert abs(float(got) - want) <= 2 * U * want
+        coef = min(1.0, float(torch.tensor(factor * want)) / (want + 1e-6))
+        for g, c in zip(grads, copies):
+            if coef == 1.0:
+                assert torch.equal(g, c)
+            else:
+                w = g.double() * coef
+                tol = w.abs() * (half(g.dtype) + 6 * U) + torch.finfo(g.dtype).smallest_normal * torch.finfo(g.dtype).eps / 2
+                assert bool(((c.double() - w).abs() <= tol).all())
+
+
+def test_views_of_a_bucket_at_every_alignment():
+    """Tensors that start at any element of a bucket; what lies between them is not touched."""
+    for dtype in TYPES:
+        flat = make([9000], 3, [dtype])[0]
+        before = flat.clone()
+        r, at, views = random.Random(1), 0, []
+        while at < 8000:
+            n = r.choice((1, 3, 8, 17, 64, 513))
+            views.append((at, n))
+            at += n + r.choice((0, 1, 2, 5))
+        grads = [flat[a:a + n] for a, n in views]
+        want = exact(grads, 2.0)
+        norm = clip_grads_(grads, 0.5 * want)
+        assert abs(float(norm) - want) <= 2 * U * want
+        mask = torch.zeros(9000, dtype=torch.bool, device="cuda")
+        for a, n in views:
+            mask[a:a + n] = True
+        assert torch.equal(flat[~mask], before[~mask])
+        w = before[mask].double() * (0.5 * want / (want + 1e-6))
+        # below its smallest normal number the type's spacing is smallest_normal * eps (float16: 2^-24, so half a step is 2^-25 = 2.98e-8)
+        least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+        assert bool(((flat[mask].double() - w).abs() <= w.abs() * (half(dtype) + 6 * U) + least).all())
+
+
+def test_orders_of_memory_and_shared_memory():
+    a = make([24], 1, [torch.float32])[0].reshape(2, 3, 4)
+    t = a.clone().permute(2, 0, 1)                          # dense in another order
+    s = make([40], 2, [torch.float32])[0].reshape(5, 8)
+    v = s[:, 2:5]                                           # not dense
+    s0, want = s.clone(), exact([a, v], 2.0)
+    assert abs(float(grad_norm([t, v])) - want) <= 2 * U * want
+    clip_grads_([t, v], 0.25 * want)
+    coef = 0.25 * want / (want + 1e-6)
+    assert torch.allclose(t, a.permute(2, 0, 1) * coef, rtol=1e-6, atol=0) and torch.allclose(v, s0[:, 2:5] * coef, rtol=1e-6, atol=0)
+    assert torch.equal(s[:, :2], s0[:, :2]) and torch.equal(s[:, 5:], s0[:, 5:])
+    flat = torch.ones(100, device="cuda")
+    assert abs(float(grad_norm([flat, flat])) - math.sqrt(200)) < 1e-5       # reading it twice is fine
+    for pair in ([flat, flat], [flat[:60], flat[59:]]):
+        with pytest.raises(IsrError, match="share memory"):
+            clip_grads_(pair, 1.0)
+    with pytest.raises(ValueError):
+        clip_grads_([torch.ones(1, device="cuda").expand(5)], 1.0)
+    assert bool((flat == 1).all())
+    assert abs(float(grad_norm([torch.ones(1, device="cuda").expand(5)])) - math.sqrt(5)) < 1e-6
+
+
+def test_large_values_long_sums_and_non_finite():
+    big = torch.full((1000,), 3e38, device="cuda")          # squares beyond 32 bits
+    assert float(grad_norm([big])) == math.inf              # beyond the largest float32
+    small = torch.full((100,), 1e25, device="cuda")
+    assert abs(float(grad_norm([small])) / 1e26 - 1) <= 4 * U
+    tiny = torch.full((100,), 1e-30, device="cuda")         # squares below 32 bits
+    assert abs(float(grad_norm([tiny])) / 1e-29 - 1) <= 4 * U
+    ones = torch.ones(2 ** 24 + 5, device="cuda")           # a sum beyond 24 bits
+    assert float(grad_norm([ones], 1.0)) == float(torch.tensor(2.0 ** 24 + 5, dtype=torch.float64).float())
+    for bad in (math.inf, math.nan):
+        for p in (2.0, 1.0, math.inf):
+            g = [torch.ones(9000, device="cuda"), torch.ones(50, device="cuda", dtype=torch.bfloat16)]
+            g[0][8500] = bad
+            n = float(grad_norm(g, p))
+            assert (math.isnan(n) if math.isnan(bad) else n == math.inf)
+            with pytest.raises(RuntimeError):
+                clip_grads_(g, 1.0, p, error_if_nonfinite=True)
+            assert float(g[0][0]) == 1.0                    # nothing was scaled
+            clip_grads_(g, 1.0, p)                          # as torch: 0 for an infinite norm, NaN for a NaN
+            assert (math.isnan(float(g[1][0])) if math.isnan(bad) else float(g[1][0]) == 0.0)
+
+
+def test_like_torch_on_parameters():
+    shapes = [(30, 7), (1,), (64, 64), (5000,)]
+    mine = [torch.nn.Parameter(torch.zeros(s, device="cuda")) for s in shapes] + [torch.nn.Parameter(torch.zeros(3, device="cuda"))]
+    theirs = [torch.nn.Parameter(torch.zeros(s, device="cuda")) for s in shapes]
+    for a, b in zip(mine, theirs):
+        a.grad = torch.randn_like(a)
+        b.grad = a.grad.clone()
+    n1, n2 = clip_grad_norm_(mine, 0.7), torch.nn.utils.clip_grad_norm_(theirs, 0.7)
+    assert abs(float(n1) - float(n2)) <= 1e-6 * float(n2)
+    for a, b in zip(mine, theirs):
+        assert torch.allclose(a.grad, b.grad, rtol=1e-6, atol=0)
+    assert mine[-1].grad is None
+    assert float(clip_grad_norm_([], 1.0)) == 0.0 and float(grad_norm([])) == 0.0
+
+
+def test_captured_and_replayed_and_on_another_stream():
+    sizes = [100, 70000, 3, 8192] * 40                      # two tables of tensors
+    grads = make(sizes, 1)
+    fresh = make(sizes, 2)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        clip_grads_([g.clone() for g in grads], 1.0)
+    torch.cuda.current_stream().wait_stream(s)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        n1 = clip_grads_(grads, 1.0)
+    with torch.cuda.graph(g2):
+        n2 = grad_norm(grads)
+    for k in range(4):
+        for a, b in zip(grads, fresh):
+            a.copy_(b * (k + 1))
+        eager = [g.clone() for g in grads]
+        g1.replay()
+        g2.replay()
+        if k % 2:
+            torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            s.wait_stream(torch.cuda.current_stream())
+            ne = clip_grads_(eager, 1.0)
+        torch.cuda.current_stream().wait_stream(s)
+        assert float(n1) == float(ne)
+        assert all(torch.equal(a, b) for a, b in zip(grads, eager))
+        assert float(n2) == float(grad_norm(eager))
+
+
+def test_more_than_2_to_the_31_elements():
+    n = 2 ** 31 + 77
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g[-3:], g[0] = 2.0, 3.0
+    assert abs(float(grad_norm([g])) - math.sqrt(21.0)) <= 1e-6
+    clip_grads_([g], 0.5 * math.sqrt(21.0))
+    assert float(g[-1]) == 1.0 and float(g[0]) == 1.5
+    del g
+    torch.cuda.empty_cache()
+
+
+def test_refusals_on_the_device():
+    x = torch.ones(4, device="cuda")
+    for call, error in [(lambda: grad_norm([x], 3.0), ValueError), (lambda: grad_norm([x.double()]), TypeError),
+                        (lambda: grad_norm([x.cpu()]), RuntimeError), (lambda: clip_grads_([x], -1.0), ValueError),
+                        (lambda: clip_grads_([x], float("nan")), ValueError), (lambda: grad_norm([x.to_sparse()]), RuntimeError)]:
+        with pytest.raises(error):
+            call()
