@@ -230,14 +230,14 @@ int iso_rms_norm_forward(int type, long long rows, int F, const void* x, long lo
 int iso_rms_norm_quant(int type, int code, long long rows, int F, int group, const void* x, long long x_stride, const void* residual,
                        long long residual_stride, const void* weight, int weight_is_float, float eps, void* codes, float* scales,
                        void* s_out, void* stream);
-/* Backward, from s (the forward's s_out, or x without a residual) and rstd:  h = s rstd,
+/* Backward, from s = x + residual (32 bits; residual may be NULL) and rstd:  h = s rstd,
  *   ds = rstd (gy weight - h mean(gy weight h)) + gs      the gradient of x and of the residual
  *   dw = sum over rows of gy h                            in weight's type; summed in 32 bits in an order that rows and F alone fix
  * gs (the gradient that reaches s_out) may be NULL; ds or dw may be NULL.  scratch: iso_rms_norm_scratch_bytes, needed with dw. */
 size_t iso_rms_norm_scratch_bytes(int type, long long rows, int F);
-int iso_rms_norm_backward(int type, long long rows, int F, const void* s, long long s_stride, const void* weight, int weight_is_float,
-                          const float* rstd, const void* gy, long long gy_stride, const void* gs, long long gs_stride, void* ds,
-                          void* dw, void* scratch, size_t scratch_bytes, void* stream);
+int iso_rms_norm_backward(int type, long long rows, int F, const void* x, long long x_stride, const void* residual, long long residual_stride,
+                          const void* weight, int weight_is_float, const float* rstd, const void* gy, long long gy_stride,
+                          const void* gs, long long gs_stride, void* ds, void* dw, void* scratch, size_t scratch_bytes, void* stream);
 
 /* A table of P rows in 8 bits: codes [P, F], scales [P, F / group], rounded per group as by iso_rms_norm_quant without a norm
  * (scale = top / Q).  Rows are written to [first, first + n) (index NULL) or to index[i] (int64 or int32): of equal indices the last one is

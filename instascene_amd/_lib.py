@@ -115,7 +115,7 @@ SIGNATURES = {
     "iso_rms_norm_quant": (c_int, [c_int, c_int, ctypes.c_longlong, c_int, c_int, _P, ctypes.c_longlong, _P, ctypes.c_longlong, _P, c_int,
                                    c_float, _P, _P, _P, _P]),
     "iso_rms_norm_scratch_bytes": (c_size_t, [c_int, ctypes.c_longlong, c_int]),
-    "iso_rms_norm_backward": (c_int, [c_int, ctypes.c_longlong, c_int, _P, ctypes.c_longlong, _P, c_int, _P, _P, ctypes.c_longlong, _P,
+    "iso_rms_norm_backward": (c_int, [c_int, ctypes.c_longlong, c_int, _P, ctypes.c_longlong, _P, ctypes.c_longlong, _P, c_int, _P, _P, ctypes.c_longlong, _P,
                                       ctypes.c_longlong, _P, _P, _P, c_size_t, _P]),
     "iso_rows8_write": (c_int, [c_int, c_int, ctypes.c_longlong, c_int, c_int, ctypes.c_longlong, _P, ctypes.c_longlong, ctypes.c_longlong,
                                 _P, c_int, _P, _P, _P, _P]),

@@ -32,6 +32,16 @@ template <class T, int N> __device__ __forceinline__ void row_load(const T* p, i
         for (int i = 0; i < N; i++) v[i] = i < left ? (float)p[i] : 0.0f;
     }
 }
+// v = x + res (res may be NULL)
+template <class T, int N> __device__ __forceinline__ void sum_load(const T* x, const T* res, int left, float (&v)[N]) {
+    row_load<T, N>(x, left, v);
+    if (res) {
+        float r[N];
+        row_load<T, N>(res, left, r);
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] += r[i];
+    }
+}
 template <class T, int N> __device__ __forceinline__ void row_store(T* p, int left, const float (&v)[N]) {
     if (left >= N) {
         typename Unaligned<T, N>::type q;
@@ -53,12 +63,50 @@ template <class T, int N> __device__ __forceinline__ void gain_load(const void* 
     else row_load<T, N>((const T*)w + at, left, v);
 }
 
-// ---- sums and maxima over the tpr threads of a row; `lds` has two slots per wave, `turn` alternates between them so that one barrier
-// per reduction is enough
+// ---- sums and maxima over the tpr threads of a row.  Within 16 lanes by DPP (quad_perm, then the mirrors of 8 and 16 lanes: every lane of
+// a half already holds its half's value), across 16 and 32 lanes by the permlane swaps: no trip through LDS.  All lanes of the wave have to
+// be active.  Between waves `lds` has two slots per wave; `turn` alternates between them so that one barrier per reduction is enough.
+template <int CTRL> __device__ __forceinline__ unsigned lane_dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+// the value of the partner at distance 1, 2, 4, 8 (STEP 0..3; 4 and 8 mirrored), 16, 32
+template <int STEP> __device__ __forceinline__ unsigned lane_partner(unsigned v) {
+    if constexpr (STEP == 0) return lane_dpp<0xB1>(v);
+    else if constexpr (STEP == 1) return lane_dpp<0x4E>(v);
+    else if constexpr (STEP == 2) return lane_dpp<0x141>(v);
+    else if constexpr (STEP == 3) return lane_dpp<0x140>(v);
+    else {
+        const bool up = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)) & (STEP == 4 ? 16u : 32u);
+        const auto q = STEP == 4 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return up ? q[0] : q[1];
+    }
+}
+template <int STEP> __device__ __forceinline__ double lane_partner(double v) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = lane_partner<STEP>((unsigned)b), hi = lane_partner<STEP>((unsigned)(b >> 32));
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+// over the lanes of aligned segments of n (a power of two) lanes of a wave
+__device__ __forceinline__ double lanes_sum(double v, int n) {
+    if (n > 1) v += lane_partner<0>(v);
+    if (n > 2) v += lane_partner<1>(v);
+    if (n > 4) v += lane_partner<2>(v);
+    if (n > 8) v += lane_partner<3>(v);
+    if (n > 16) v += lane_partner<4>(v);
+    if (n > 32) v += lane_partner<5>(v);
+    return v;
+}
+__device__ __forceinline__ unsigned lanes_max(unsigned v, int n) {
+    if (n > 1) v = max(v, lane_partner<0>(v));
+    if (n > 2) v = max(v, lane_partner<1>(v));
+    if (n > 4) v = max(v, lane_partner<2>(v));
+    if (n > 8) v = max(v, lane_partner<3>(v));
+    if (n > 16) v = max(v, lane_partner<4>(v));
+    if (n > 32) v = max(v, lane_partner<5>(v));
+    return v;
+}
 __device__ __forceinline__ double row_sum(double v, int tpr, double (*lds)[16], int turn) {
-    for (int o = min(tpr, 64) >> 1; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    v = lanes_sum(v, tpr);
     if (tpr > 64) {
-        const int wave = threadIdx.x >> 6, first = (threadIdx.x / tpr) * (tpr >> 6), n = tpr >> 6;
+        const int wave = threadIdx.x >> 6, n = tpr >> 6, first = wave & ~(n - 1);
         if ((threadIdx.x & 63) == 0) lds[turn][wave] = v;
         __syncthreads();
         v = 0.0;
@@ -67,9 +115,9 @@ __device__ __forceinline__ double row_sum(double v, int tpr, double (*lds)[16], 
     return v;
 }
 __device__ __forceinline__ unsigned row_max(unsigned v, int tpr, double (*lds)[16], int turn) {
-    for (int o = min(tpr, 64) >> 1; o >= 1; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
+    v = lanes_max(v, tpr);
     if (tpr > 64) {
-        const int wave = threadIdx.x >> 6, first = (threadIdx.x / tpr) * (tpr >> 6), n = tpr >> 6;
+        const int wave = threadIdx.x >> 6, n = tpr >> 6, first = wave & ~(n - 1);
         if ((threadIdx.x & 63) == 0) lds[turn][wave] = (double)v;          // (exact: 32 bits)
         __syncthreads();
         v = 0;
@@ -90,10 +138,10 @@ template <int CODE> struct Code8;
 template <> struct Code8<CODE_INT8> {
     static constexpr float Q = 127.0f;
     static __device__ __forceinline__ unsigned pack4(const float* p) {
-        unsigned r = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) r |= ((unsigned)(int)__builtin_rintf(p[i]) & 0xffu) << (8 * i);
-        return r;
+        // + 1.5 2^23 rounds to a whole number, ties to even, whose low byte is the code
+        const unsigned a = __float_as_uint(p[0] + 12582912.0f), b = __float_as_uint(p[1] + 12582912.0f);
+        const unsigned c = __float_as_uint(p[2] + 12582912.0f), d = __float_as_uint(p[3] + 12582912.0f);
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
     }
     static __device__ __forceinline__ float one(unsigned c) { return (float)(signed char)c; }
     static __device__ __forceinline__ void unpack4(unsigned c, float* v) {
@@ -114,34 +162,46 @@ template <> struct Code8<CODE_E4M3> {
     }
 };
 
+// What encodes a group: its largest magnitude, Q / top a little below and above, the scale top / Q.
+struct Group8 { float top, lo, hi, scale; };
+// From the bits of the largest magnitude.  Q / top by v_rcp_f32 (within 2^-21.6 with the roundings around it; encode4 allows 2^-21), top / Q correctly rounded: the
+// product with 1 / Q, corrected once by its exact remainder.
+template <int CODE> __device__ __forceinline__ Group8 group_scale(unsigned top_bits) {
+    constexpr float Q = Code8<CODE>::Q, rq = 1.0f / Q;
+    Group8 g;
+    g.top = __uint_as_float(top_bits);
+    const float s = g.top * rq, inv = __builtin_amdgcn_rcpf(s);         // (of top / Q: of top itself it would be below the normal numbers)
+    g.lo = inv * (1.0f - 0x1p-21f);
+    g.hi = inv * (1.0f + 0x1p-21f);
+    g.scale = __builtin_fmaf(__builtin_fmaf(-s, Q, g.top), rq, s);
+    if (g.top < ROWS_TINY || top_bits >= 0x7f800000u) {
+        g.lo = g.hi = 0.0f;
+        g.scale = top_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : 0.0f;      // an infinity or NaN: the group reads back as NaN
+    }
+    return g;
+}
 // The codes of four values of a group: t Q / top rounded to the nearest code, ties to even, as if the quotient were exact.  The 32-bit
-// product t (Q / top) is off by at most 2^-23 of itself; where a border between two codes lies that near (the codes of the
-// product scaled by 1 -+ 2^-21 differ: one value in 1e5) both sides of the comparison |t| Q <> border top are formed exactly in 64 bits.
-template <int CODE> __device__ __forceinline__ unsigned encode4(const float* t, float inv, float top) {
+// products t lo and t hi bracket it; where they round to different codes (one value in 1e5) a border lies between them, and both sides of
+// |t| Q <> border top are formed exactly in 64 bits.
+template <int CODE> __device__ __forceinline__ unsigned encode4(const float* t, const Group8& g) {
     using C = Code8<CODE>;
-    float p[4], lo[4], hi[4];
+    float lo[4], hi[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) { p[i] = inv > 0.0f ? t[i] * inv : 0.0f; lo[i] = p[i] * (1.0f - 0x1p-21f); hi[i] = p[i] * (1.0f + 0x1p-21f); }
+    for (int i = 0; i < 4; i++) { lo[i] = t[i] * g.lo; hi[i] = t[i] * g.hi; }
     unsigned in = C::pack4(lo);
     const unsigned out = C::pack4(hi);
+    if (g.hi == 0.0f) return 0;                 // (an infinity or NaN times 0)
     if (in != out) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const unsigned a = (in >> (8 * i)) & 0xffu, b = (out >> (8 * i)) & 0xffu;
             if (a == b) continue;
-            const double border = 0.5 * (fabs((double)C::one(a)) + fabs((double)C::one(b))) * (double)top;
+            const double border = 0.5 * (fabs((double)C::one(a)) + fabs((double)C::one(b))) * (double)g.top;
             const double value = fabs((double)t[i]) * (double)C::Q;
             if (value > border || (value == border && (a & 1u))) in = (in & ~(0xffu << (8 * i))) | (b << (8 * i));
         }
     }
     return in;
-}
-// Q / top and top / Q of a group from the bits of its largest magnitude
-template <int CODE> __device__ __forceinline__ void group_scale(unsigned top_bits, float& top, float& inv, float& scale) {
-    top = __uint_as_float(top_bits);
-    if (top_bits >= 0x7f800000u) { inv = 0.0f; scale = __uint_as_float(0x7fc00000u); }        // an infinity or NaN: the group reads back as NaN
-    else if (top < ROWS_TINY) { inv = 0.0f; scale = 0.0f; }
-    else { inv = Code8<CODE>::Q / top; scale = top / Code8<CODE>::Q; }
 }
 template <int N> __device__ __forceinline__ void code_store(unsigned char* p, int left, const unsigned (&c)[N / 4]) {
     if (left >= N) __builtin_memcpy(p, c, N);
@@ -194,7 +254,7 @@ __device__ __forceinline__ long long row_target(const RowTarget& d, long long i,
 // OUT = 0: y in T, else codes and scales.  norm = 0: no statistics (rstd = 1), the plain writing of a table.
 struct RmsArgs {
     long long rows, row0;   // this launch starts at row row0
-    int F, tpr, norm, w32;
+    int F, tpr, tsh, norm, w32;     // tpr = 1 << tsh threads per row
     int groups, gshift;     // groups per row and log2 of their columns; one group: 1 and 31
     float eps;
     double inv_F;
@@ -214,7 +274,7 @@ template <class T, int NV, int OUT> __global__ __launch_bounds__(512) void rms_f
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1);
-    const long long i = a.row0 + (long long)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+    const long long i = a.row0 + (long long)blockIdx.x * (blockDim.x >> a.tsh) + (threadIdx.x >> a.tsh);
     const bool on = i < a.rows;
     const T* x = (const T*)a.x + (on ? i : 0) * a.ldx;
     const T* res = a.res ? (const T*)a.res + (on ? i : 0) * a.ldr : nullptr;
@@ -228,13 +288,7 @@ template <class T, int NV, int OUT> __global__ __launch_bounds__(512) void rms_f
             for (int e = 0; e < N; e++) v[k][e] = 0.0f;
             continue;
         }
-        row_load<T, N>(x + at, left, v[k]);
-        if (res) {
-            float r[N];
-            row_load<T, N>(res + at, left, r);
-#pragma unroll
-            for (int e = 0; e < N; e++) v[k][e] += r[e];
-        }
+        sum_load<T, N>(x + at, res ? res + at : nullptr, left, v[k]);
     }
     if (a.norm) {
 #pragma unroll
@@ -274,16 +328,15 @@ template <class T, int NV, int OUT> __global__ __launch_bounds__(512) void rms_f
                 top_bits = 0;
 #pragma unroll
                 for (int e = 0; e < N; e++) top_bits = max(top_bits, __float_as_uint(v[k][e]) & 0x7fffffffu);
-                for (int o = seg >> 1; o >= 1; o >>= 1) top_bits = max(top_bits, (unsigned)__shfl_xor((int)top_bits, o));
+                top_bits = lanes_max(top_bits, seg);
             }
-            float top, inv, scale;
-            group_scale<OUT>(top_bits, top, inv, scale);
+            const Group8 g = group_scale<OUT>(top_bits);
             if (row < 0 || left <= 0) continue;
             unsigned c[N / 4];
 #pragma unroll
-            for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[k][4 * q], inv, top);
+            for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[k][4 * q], g);
             code_store<N>(a.codes + row * a.F + at, left, c);
-            if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = scale * rstd;
+            if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
         }
     }
 }
@@ -301,13 +354,8 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
     unsigned row_top = 0;
     const bool by_row = OUT != 0 && a.groups == 1;
     for (int at = t * N; at < a.F; at += tpr * N) {
-        float v[N], r[N], w[N];
-        row_load<T, N>(x + at, a.F - at, v);
-        if (res) {
-            row_load<T, N>(res + at, a.F - at, r);
-#pragma unroll
-            for (int e = 0; e < N; e++) v[e] += r[e];
-        }
+        float v[N], w[N];
+        sum_load<T, N>(x + at, res ? res + at : nullptr, a.F - at, v);
 #pragma unroll
         for (int e = 0; e < N; e++) ss += (double)v[e] * (double)v[e];
         if (by_row) {
@@ -324,13 +372,8 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
     // (all threads of a wave take every step together: the groups' maxima are shuffled)
     for (int base = 0; base < a.F; base += tpr * N) {
         const int at = base + t * N, left = a.F - at;
-        float v[N], r[N], w[N];
-        row_load<T, N>(x + (left > 0 ? at : 0), left > 0 ? left : 0, v);
-        if (res) {
-            row_load<T, N>(res + (left > 0 ? at : 0), left > 0 ? left : 0, r);
-#pragma unroll
-            for (int e = 0; e < N; e++) v[e] += r[e];
-        }
+        float v[N], w[N];
+        sum_load<T, N>(x + at, res ? res + at : nullptr, left, v);          // (left <= 0: nothing is read)
         if (a.s && left > 0) row_store<T, N>((T*)a.s + i * a.F + at, left, v);
         if (left > 0) gain_load<T, N>(a.w, a.w32, at, left, w);
         else {
@@ -347,16 +390,15 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
                 top_bits = 0;
 #pragma unroll
                 for (int e = 0; e < N; e++) top_bits = max(top_bits, __float_as_uint(v[e]) & 0x7fffffffu);
-                for (int o = seg >> 1; o >= 1; o >>= 1) top_bits = max(top_bits, (unsigned)__shfl_xor((int)top_bits, o));
+                top_bits = lanes_max(top_bits, seg);
             }
-            float top, inv, scale;
-            group_scale<OUT>(top_bits, top, inv, scale);
+            const Group8 g = group_scale<OUT>(top_bits);
             if (row >= 0 && left > 0) {
                 unsigned c[N / 4];
 #pragma unroll
-                for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[4 * q], inv, top);
+                for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[4 * q], g);
                 code_store<N>(a.codes + row * a.F + at, left, c);
-                if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = scale * rstd;
+                if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
             }
         }
     }
@@ -365,9 +407,11 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
 // ---- backward --------------------------------------------------------------------------------------------------------------------
 struct RmsBackArgs {
     long long rows, row0;   // row0: of the *_long kernel
-    int F, tpr, w32;
-    const void* s;
-    long long lds_;
+    int F, tpr, tsh, w32;
+    const void* x;          // s = x + res
+    long long ldx;
+    const void* res;        // or NULL
+    long long ldr;
     const void* w;          // or NULL
     const float* rstd;
     const void* gy;
@@ -381,7 +425,7 @@ template <class T, int NV> __global__ __launch_bounds__(512) void rms_backward_k
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     __shared__ float part[8][64 * N];       // the waves' sums of one vector slot
-    const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), rpb = blockDim.x / tpr;
+    const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), rpb = blockDim.x >> a.tsh;
     float dw[NV][N], w[NV][N];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
@@ -392,10 +436,11 @@ template <class T, int NV> __global__ __launch_bounds__(512) void rms_backward_k
     }
     int turn = 0;
     for (long long r0 = (long long)blockIdx.x * rpb; r0 < a.rows; r0 += (long long)gridDim.x * rpb, turn ^= 1) {
-        const long long i = r0 + threadIdx.x / tpr;
+        const long long i = r0 + (threadIdx.x >> a.tsh);
         const bool on = i < a.rows;
         const float rstd = on ? a.rstd[i] : 0.0f;
-        const T* s = (const T*)a.s + (on ? i : 0) * a.lds_;
+        const T* x = (const T*)a.x + (on ? i : 0) * a.ldx;
+        const T* res = a.res ? (const T*)a.res + (on ? i : 0) * a.ldr : nullptr;
         const T* gy = (const T*)a.gy + (on ? i : 0) * a.ldg;
         float h[NV][N], g[NV][N];
         float c = 0.0f;
@@ -405,7 +450,7 @@ template <class T, int NV> __global__ __launch_bounds__(512) void rms_backward_k
 #pragma unroll
             for (int e = 0; e < N; e++) { h[k][e] = 0.0f; g[k][e] = 0.0f; }
             if (left <= 0) continue;
-            row_load<T, N>(s + at, left, h[k]);
+            sum_load<T, N>(x + at, res ? res + at : nullptr, left, h[k]);
             row_load<T, N>(gy + at, left, g[k]);
         }
 #pragma unroll
@@ -471,13 +516,14 @@ template <class T> __global__ __launch_bounds__(512) void rms_backward_long_kern
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x;
     const long long i = a.row0 + blockIdx.x;
-    const T* s = (const T*)a.s + i * a.lds_;
+    const T* x = (const T*)a.x + i * a.ldx;
+    const T* res = a.res ? (const T*)a.res + i * a.ldr : nullptr;
     const T* gy = (const T*)a.gy + i * a.ldg;
     const float rstd = a.rstd[i];
     double c = 0.0;
     for (int at = t * N; at < a.F; at += tpr * N) {
         float h[N], g[N], w[N];
-        row_load<T, N>(s + at, a.F - at, h);
+        sum_load<T, N>(x + at, res ? res + at : nullptr, a.F - at, h);
         row_load<T, N>(gy + at, a.F - at, g);
         gain_load<T, N>(a.w, a.w32, at, a.F - at, w);
         float p = 0.0f;
@@ -489,7 +535,7 @@ template <class T> __global__ __launch_bounds__(512) void rms_backward_long_kern
     const float mean = (float)row_sum(c, tpr, lds, 0) / (float)a.F;
     for (int at = t * N; at < a.F; at += tpr * N) {
         float h[N], g[N], w[N], d[N];
-        row_load<T, N>(s + at, a.F - at, h);
+        sum_load<T, N>(x + at, res ? res + at : nullptr, a.F - at, h);
         row_load<T, N>(gy + at, a.F - at, g);
         gain_load<T, N>(a.w, a.w32, at, a.F - at, w);
 #pragma unroll
@@ -507,22 +553,32 @@ template <class T> __global__ __launch_bounds__(256) void rms_dw_columns_kernel(
     const long long col = (long long)blockIdx.x * 256 + threadIdx.x;
     if (col >= a.F) return;
     float sum = 0.0f;
-    for (long long i = blockIdx.y; i < a.rows; i += slices)
-        sum += (float)((const T*)a.gy)[i * a.ldg + col] * ((float)((const T*)a.s)[i * a.lds_ + col] * a.rstd[i]);
+    for (long long i = blockIdx.y; i < a.rows; i += slices) {
+        float v = (float)((const T*)a.x)[i * a.ldx + col];
+        if (a.res) v += (float)((const T*)a.res)[i * a.ldr + col];
+        sum += (float)((const T*)a.gy)[i * a.ldg + col] * (v * a.rstd[i]);
+    }
     a.dw_part[(long long)blockIdx.y * a.F + col] = sum;
 }
-// dw = the sum of n partial rows, in a fixed order: 32 columns and 8 slices of the partials per workgroup
-template <class T> __global__ __launch_bounds__(256) void rms_dw_sum_kernel(int F, int n, const float* __restrict__ part, T* __restrict__ dw) {
-    __shared__ float lds[8][33];
+// dw = the sum of n partial rows, in a fixed order: 32 columns and 32 slices of the partials per workgroup, eight loads in flight each (a
+// narrow table has one workgroup here and up to 2048 partials: what counts is the number of loads that wait for each other)
+template <class T> __global__ __launch_bounds__(1024) void rms_dw_sum_kernel(int F, int n, const float* __restrict__ part, T* __restrict__ dw) {
+    __shared__ float lds[32][33];
     const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
     const long long col = (long long)blockIdx.x * 32 + c;
     float sum = 0.0f;
     if (col < F)
-        for (int i = q; i < n; i += 8) sum += part[(long long)i * F + col];
+        for (int i = q; i < n; i += 256) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] = i + 32 * u < n ? part[(long long)(i + 32 * u) * F + col] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; u++) sum += v[u];
+        }
     lds[q][c] = sum;
     __syncthreads();
     if (q == 0 && col < F) {
-        for (int i = 1; i < 8; i++) sum += lds[i][c];
+        for (int i = 1; i < 32; i++) sum += lds[i][c];
         dw[col] = (T)sum;
     }
 }
@@ -531,22 +587,22 @@ template <class T> __global__ __launch_bounds__(256) void rms_dw_sum_kernel(int 
 // out[i] = the values of row (first + i | index[i]); norm: divided by (|row|_2 + eps).  Rows outside [0, P) are zeros.
 struct ReadArgs {
     long long rows, row0, P, first;
-    int F, tpr, groups, gshift, norm, is64;
+    int F, tpr, tsh, groups, gshift, norm, is64;
     float eps;
     const unsigned char* codes;
     const float* scales;
     const void* index;      // or NULL
     void* out;              // [rows, F]
 };
-template <int CODE> __device__ __forceinline__ void code_load(const unsigned char* p, int left, float (&v)[8]) {
-    if (left >= 8) {
-        unsigned c[2];
-        __builtin_memcpy(c, p, 8);
-        Code8<CODE>::unpack4(c[0], v);
-        Code8<CODE>::unpack4(c[1], v + 4);
+template <int CODE, int N> __device__ __forceinline__ void code_load(const unsigned char* p, int left, float (&v)[N]) {
+    if (left >= N) {
+        unsigned c[N / 4];
+        __builtin_memcpy(c, p, N);
+#pragma unroll
+        for (int q = 0; q < N / 4; q++) Code8<CODE>::unpack4(c[q], v + 4 * q);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = e < left ? Code8<CODE>::one(p[e]) : 0.0f;
+        for (int e = 0; e < N; e++) v[e] = e < left ? Code8<CODE>::one(p[e]) : 0.0f;
     }
 }
 __device__ __forceinline__ float l2_inverse(double ss, float eps) {
@@ -554,24 +610,25 @@ __device__ __forceinline__ float l2_inverse(double ss, float eps) {
     return 1.0f / (n + eps);
 }
 template <class T, int CODE, int NV> __global__ __launch_bounds__(512) void rows_read_kernel(ReadArgs a) {
+    constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1);
-    const long long i = a.row0 + (long long)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+    const long long i = a.row0 + (long long)blockIdx.x * (blockDim.x >> a.tsh) + (threadIdx.x >> a.tsh);
     long long row = -1;
     if (i < a.rows) row = a.index == nullptr ? a.first + i : a.is64 ? ((const long long*)a.index)[i] : (long long)((const int*)a.index)[i];
     if (row >= a.P) row = -1;
-    float v[NV][8];
+    float v[NV][N];
     double ss = 0.0;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        const int at = (t + k * tpr) * 8, left = row >= 0 ? a.F - at : 0;
+        const int at = (t + k * tpr) * N, left = row >= 0 ? a.F - at : 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[k][e] = 0.0f;
+        for (int e = 0; e < N; e++) v[k][e] = 0.0f;
         if (left <= 0) continue;
-        code_load<CODE>(a.codes + row * a.F + at, left, v[k]);
+        code_load<CODE, N>(a.codes + row * a.F + at, left, v[k]);
         const float scale = a.scales[row * a.groups + (at >> a.gshift)];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
+        for (int e = 0; e < N; e++) {
             v[k][e] = e < left ? v[k][e] * scale : 0.0f;
             ss += (double)v[k][e] * (double)v[k][e];
         }
@@ -582,14 +639,15 @@ template <class T, int CODE, int NV> __global__ __launch_bounds__(512) void rows
     if (i >= a.rows) return;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        const int at = (t + k * tpr) * 8, left = a.F - at;
+        const int at = (t + k * tpr) * N, left = a.F - at;
         if (left <= 0) continue;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[k][e] *= inv;
-        row_store<T, 8>((T*)a.out + i * a.F + at, left, v[k]);
+        for (int e = 0; e < N; e++) v[k][e] *= inv;
+        row_store<T, N>((T*)a.out + i * a.F + at, left, v[k]);
     }
 }
 template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_long_kernel(ReadArgs a) {
+    constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x;
     const long long i = a.row0 + blockIdx.x;
@@ -599,27 +657,27 @@ template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_lo
     if (a.norm) {
         double ss = 0.0;
         if (row >= 0)
-            for (int at = t * 8; at < a.F; at += tpr * 8) {
-                float v[8];
-                code_load<CODE>(a.codes + row * a.F + at, a.F - at, v);
+            for (int at = t * N; at < a.F; at += tpr * N) {
+                float v[N];
+                code_load<CODE, N>(a.codes + row * a.F + at, a.F - at, v);
                 const float scale = a.scales[row * a.groups + (at >> a.gshift)];
 #pragma unroll
-                for (int e = 0; e < 8; e++)
+                for (int e = 0; e < N; e++)
                     if (at + e < a.F) ss += (double)(v[e] * scale) * (double)(v[e] * scale);
             }
         inv = l2_inverse(row_sum(ss, tpr, lds, 0), a.eps);
     }
-    for (int at = t * 8; at < a.F; at += tpr * 8) {
-        float v[8];
+    for (int at = t * N; at < a.F; at += tpr * N) {
+        float v[N];
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = 0.0f;
+        for (int e = 0; e < N; e++) v[e] = 0.0f;
         if (row >= 0) {
-            code_load<CODE>(a.codes + row * a.F + at, a.F - at, v);
+            code_load<CODE, N>(a.codes + row * a.F + at, a.F - at, v);
             const float scale = a.scales[row * a.groups + (at >> a.gshift)];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = v[e] * scale * inv;
+            for (int e = 0; e < N; e++) v[e] = v[e] * scale * inv;
         }
-        row_store<T, 8>((T*)a.out + i * a.F + at, a.F - at, v);
+        row_store<T, N>((T*)a.out + i * a.F + at, a.F - at, v);
     }
 }
 

@@ -19,17 +19,18 @@ bool code_type(int c) { return c == iso::CODE_INT8 || c == iso::CODE_E4M3; }
 bool group_ok(int F, int group) { return group == F || ((group == 32 || group == 64 || group == 128) && F % group == 0); }
 int group_shift(int F, int group) { return group == F ? 31 : group == 32 ? 5 : group == 64 ? 6 : 7; }
 
-// threads per row (a power of two) and vectors per thread for a row of `vecs` vectors; 0 vectors per thread: the *_long form.
-// A wave and fewer as long as 4 vectors per thread do (no barrier between waves); beyond, or where there are so few rows that
-// the chip would stand idle, up to 512 threads.
-void row_shape(int vecs, long long rows, int max_nv, int& tpr, int& nv) {
-    tpr = 1;
-    while (tpr < vecs && tpr < 64) tpr <<= 1;
-    while (tpr < 512 && tpr < vecs && ((vecs + tpr - 1) / tpr > 4 || rows * tpr < 256 * 256)) tpr <<= 1;
-    const int need = (vecs + tpr - 1) / tpr;
+// threads per row (1 << tsh) and vectors per thread for a row of `vecs` vectors; 0 vectors per thread: the *_long form.
+// A wave and fewer as long as 4 vectors per thread do (no barrier between waves), `least` vectors per thread where the row has them and there
+// are rows enough to fill the chip; where the chip would stand idle, or beyond 4 vectors in a wave, up to 512 threads.
+void row_shape(int vecs, long long rows, int least, int max_nv, int& tsh, int& nv) {
+    tsh = 0;
+    while ((1 << tsh) < vecs && tsh < 6) tsh++;
+    while (tsh > 0 && (1 << tsh) * least > vecs && (1 << (tsh - 1)) * least >= vecs && (rows << (tsh - 1)) >= 2048 * 256) tsh--;
+    while (tsh < 9 && (1 << tsh) < vecs && ((vecs + (1 << tsh) - 1) >> tsh > 4 || (rows << tsh) < 256 * 256)) tsh++;
+    const int need = (vecs + (1 << tsh) - 1) >> tsh;
     nv = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : need <= 8 ? 8 : 0;
     if (nv > max_nv) nv = 0;
-    if (nv == 0) tpr = 512;
+    if (nv == 0) tsh = 9;
 }
 
 #define ROWS_NV(nv, call_nv, call_long) \
@@ -37,7 +38,8 @@ void row_shape(int vecs, long long rows, int max_nv, int& tpr, int& nv) {
 
 template <class T, int OUT> void launch_forward(iso::RmsArgs a, hipStream_t s) {
     int nv;
-    row_shape((a.F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, a.rows, 8, a.tpr, nv);
+    row_shape((a.F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, a.rows, OUT == 0 ? 1 : 2, 8, a.tsh, nv);
+    a.tpr = 1 << a.tsh;
     const int block = std::max(256, a.tpr);
     const long long step = MAX_THREADS / block * (block / a.tpr);
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
@@ -61,18 +63,19 @@ void launch_codes(int code, int type, const iso::RmsArgs& a, hipStream_t s) {
 }
 
 // workgroups of the backward pass = partial rows of dw: enough to fill the chip, few enough that the partials stay small against the rows
-template <class T> void backward_shape(long long rows, int F, int& tpr, int& nv, int& block, int& grid) {
-    row_shape((F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, rows, 4, tpr, nv);
+template <class T> void backward_shape(long long rows, int F, int& tsh, int& nv, int& block, int& grid) {
+    row_shape((F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, rows, 1, 4, tsh, nv);
+    const int tpr = 1 << tsh;
     block = std::max(256, tpr);
     if (nv == 0) { grid = (int)std::min<long long>(64, std::max<long long>(1, rows)); return; }       // slices of the columns' sums
     const long long need = (rows + block / tpr - 1) / (block / tpr);
     const long long most = std::max<long long>(512, std::min<long long>(2048, (1 << 20) / F));
     grid = (int)std::max<long long>(1, std::min(need, most));
 }
-void backward_shape_type(int type, long long rows, int F, int& tpr, int& nv, int& block, int& grid) {
-    if (type == 0) backward_shape<float>(rows, F, tpr, nv, block, grid);
-    else if (type == 1) backward_shape<__bf16>(rows, F, tpr, nv, block, grid);
-    else backward_shape<_Float16>(rows, F, tpr, nv, block, grid);
+void backward_shape_type(int type, long long rows, int F, int& tsh, int& nv, int& block, int& grid) {
+    if (type == 0) backward_shape<float>(rows, F, tsh, nv, block, grid);
+    else if (type == 1) backward_shape<__bf16>(rows, F, tsh, nv, block, grid);
+    else backward_shape<_Float16>(rows, F, tsh, nv, block, grid);
 }
 template <class T> void launch_backward(iso::RmsBackArgs a, int nv, int block, int grid, hipStream_t s) {
     if (nv == 1) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 1>), dim3(grid), dim3(block), 0, s, a);
@@ -87,7 +90,8 @@ template <class T> void launch_backward(iso::RmsBackArgs a, int nv, int block, i
 }
 template <class T, int CODE> void launch_read(iso::ReadArgs a, hipStream_t s) {
     int nv;
-    row_shape((a.F + 7) / 8, a.rows, 8, a.tpr, nv);
+    row_shape((a.F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, a.rows, 2, 8, a.tsh, nv);
+    a.tpr = 1 << a.tsh;
     const int block = std::max(256, a.tpr);
     const long long step = MAX_THREADS / block * (block / a.tpr);
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
@@ -149,33 +153,35 @@ int iso_rms_norm_quant(int type, int code, long long rows, int F, int group, con
 
 size_t iso_rms_norm_scratch_bytes(int type, long long rows, int F) {
     if (!row_type(type) || rows <= 0 || F < 1 || F > (1 << 24)) return 0;
-    int tpr, nv, block, grid;
-    backward_shape_type(type, rows, F, tpr, nv, block, grid);
+    int tsh, nv, block, grid;
+    backward_shape_type(type, rows, F, tsh, nv, block, grid);
     return (size_t)grid * (size_t)F * sizeof(float);
 }
 
-int iso_rms_norm_backward(int type, long long rows, int F, const void* s_in, long long s_stride, const void* weight, int weight_is_float,
+int iso_rms_norm_backward(int type, long long rows, int F, const void* x, long long x_stride, const void* residual,
+                          long long residual_stride, const void* weight, int weight_is_float,
                           const float* rstd, const void* gy, long long gy_stride, const void* gs, long long gs_stride, void* ds,
                           void* dw, void* scratch, size_t scratch_bytes, void* stream) {
     if (const int e = check_rows("rms_norm_backward", type, rows, F)) return e;
     hipStream_t s = (hipStream_t)stream;
     if (rows == 0) return ISR_OK;
-    if (!s_in || !rstd || !gy || (!ds && !dw)) return fail(ISR_EINVAL, "rms_norm_backward: null pointer");
+    if (!x || !rstd || !gy || (!ds && !dw)) return fail(ISR_EINVAL, "rms_norm_backward: null pointer");
     if (dw && (!scratch || scratch_bytes < iso_rms_norm_scratch_bytes(type, rows, F))) return fail(ISR_EINVAL, "rms_norm_backward: scratch too small");
     iso::RmsBackArgs a = {};
-    a.rows = rows; a.F = F; a.w32 = weight_is_float; a.s = s_in; a.lds_ = s_stride; a.w = weight; a.rstd = rstd;
+    a.rows = rows; a.F = F; a.w32 = weight_is_float; a.x = x; a.ldx = x_stride; a.res = residual; a.ldr = residual_stride; a.w = weight; a.rstd = rstd;
     a.gy = gy; a.ldg = gy_stride; a.gs = gs; a.ldgs = gs_stride; a.ds = ds; a.dw_part = dw ? (float*)scratch : nullptr;
     int nv, block, grid;
-    backward_shape_type(type, rows, F, a.tpr, nv, block, grid);
+    backward_shape_type(type, rows, F, a.tsh, nv, block, grid);
+    a.tpr = 1 << a.tsh;
     if (type == 0) launch_backward<float>(a, nv, block, grid, s);
     else if (type == 1) launch_backward<__bf16>(a, nv, block, grid, s);
     else launch_backward<_Float16>(a, nv, block, grid, s);
     ISR_LAUNCH_CHECK("iso_rms_norm_backward");
     if (dw) {
         const dim3 cols((F + 31) / 32);
-        if (weight_is_float || type == 0) hipLaunchKernelGGL((iso::rms_dw_sum_kernel<float>), cols, dim3(256), 0, s, F, grid, (const float*)scratch, (float*)dw);
-        else if (type == 1) hipLaunchKernelGGL((iso::rms_dw_sum_kernel<__bf16>), cols, dim3(256), 0, s, F, grid, (const float*)scratch, (__bf16*)dw);
-        else hipLaunchKernelGGL((iso::rms_dw_sum_kernel<_Float16>), cols, dim3(256), 0, s, F, grid, (const float*)scratch, (_Float16*)dw);
+        if (weight_is_float || type == 0) hipLaunchKernelGGL((iso::rms_dw_sum_kernel<float>), cols, dim3(1024), 0, s, F, grid, (const float*)scratch, (float*)dw);
+        else if (type == 1) hipLaunchKernelGGL((iso::rms_dw_sum_kernel<__bf16>), cols, dim3(1024), 0, s, F, grid, (const float*)scratch, (__bf16*)dw);
+        else hipLaunchKernelGGL((iso::rms_dw_sum_kernel<_Float16>), cols, dim3(1024), 0, s, F, grid, (const float*)scratch, (_Float16*)dw);
         ISR_LAUNCH_CHECK("iso_rms_norm_backward");
     }
     return ISR_OK;

@@ -80,23 +80,29 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps, residual):
         y, s, rstd = _forward(x, weight, eps, residual, True)
-        ctx.save_for_backward(x if s is None else s, weight, rstd)
+        # float32: s is x + residual exactly as the norm took it.  16 bits: s was rounded once more on its way out, and the gradient
+        # of the weight would carry that (2^-9 of every term): x and the residual are read again instead
+        if s is None or x.dtype == torch.float32:
+            ctx.save_for_backward(x if s is None else s, None, weight, rstd)
+        else:
+            ctx.save_for_backward(x, residual, weight, rstd)
         ctx.set_materialize_grads(False)
         return y if s is None else (y, s)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy, gs=None):
-        s, weight, rstd = ctx.saved_tensors
+        x, residual, weight, rstd = ctx.saved_tensors
         need_x, need_w, _, need_r = ctx.needs_input_grad
         if gy is None:                                    # only the sum was used: its gradient passes through
             return (gs if need_x else None), None, None, (gs if need_r else None)
-        L, dev = lib(), s.device
-        s2, g2 = _rows2d(s), _rows2d(gy)
+        L, dev = lib(), x.device
+        x2, g2 = _rows2d(x), _rows2d(gy)
+        r2 = None if residual is None else _rows2d(residual)
         q2 = None if gs is None else _rows2d(gs)
-        n, F = s2.shape
-        kind = ROW_TYPES[s.dtype]
-        ds = torch.empty(s.shape, dtype=s.dtype, device=dev) if need_x or need_r else None
+        n, F = x2.shape
+        kind = ROW_TYPES[x.dtype]
+        ds = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x or need_r else None
         dw = scratch = w = None
         nbytes = 0
         if weight is not None:
@@ -108,8 +114,8 @@ class _RmsNorm(torch.autograd.Function):
         if ds is None and dw is None:
             return None, None, None, None
         with _hot.on_device(dev):
-            check(L.iso_rms_norm_backward(kind, n, F, _p(s2), s2.stride(0), _p(w), int(w is not None and w.dtype == torch.float32), _p(rstd),
-                                          _p(g2), g2.stride(0), _p(q2), 0 if q2 is None else q2.stride(0), _p(ds), _p(dw), _p(scratch), nbytes,
+            check(L.iso_rms_norm_backward(kind, n, F, _p(x2), x2.stride(0), _p(r2), 0 if r2 is None else r2.stride(0), _p(w),
+                                          int(w is not None and w.dtype == torch.float32), _p(rstd), _p(g2), g2.stride(0), _p(q2), 0 if q2 is None else q2.stride(0), _p(ds), _p(dw), _p(scratch), nbytes,
                                           _hot.raw_stream(dev)), "iso_rms_norm_backward")
         return (ds if need_x else None), dw, None, (ds if need_r else None)
 
@@ -118,7 +124,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     """``y = s / sqrt(mean(s^2) + eps) * weight`` over the last dimension, ``s = x + residual``; returns ``y``, or ``(y, s)`` with a
     residual.  float32, bfloat16 or float16, rows of any width and stride; everything between input and output is held in 32 bits
     (the sum of squares in 64), ``y`` and ``s`` are rounded once.  ``weight`` is float32 or of x's type.  Differentiable in ``x``,
-    ``weight`` and ``residual`` (the backward pass reads ``s`` as it was returned, i.e. rounded to x's type)."""
+    ``weight`` and ``residual``."""
     _check_norm("rms_norm", x, weight, eps, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (residual is not None and residual.requires_grad)):

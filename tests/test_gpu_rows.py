@@ -72,8 +72,7 @@ def test_rms_norm_forward_and_backward(dtype, width, rows, residual, gain):
     grads = torch.autograd.grad((y, s) if residual else y, inputs, (gy, gs) if residual else gy)
     grads = dict(zip([n for n, t in (("x", x), ("r", r), ("w", w)) if t is not None], grads))
     with torch.no_grad():
-        # from s as it was returned (rounded to its type) and the statistics of the unrounded one
-        h = (s.double() if residual else x.double()) * rstd
+        h = s64 * rstd
         gw = gy.double() * (1.0 if w is None else w.double())
         mean = (gw * h).mean(dim=1, keepdim=True)
         ds = rstd * (gw - h * mean) + (gs.double() if residual else 0.0)
@@ -120,7 +119,7 @@ def test_rms_norm_backward_long_sums_and_partial_gradients():
     both = torch.autograd.grad(y, (x, w), gy)
     assert torch.equal(dw, both[1]) and torch.equal(dx, both[0])
     s64, rstd, _ = norm_reference(x.detach(), None, 1e-6, r)
-    h = s.detach().double() * rstd
+    h = s64 * rstd
     check(dw, (gy.double() * h).sum(0), (gy.double() * h).abs().sum(0) * 512 * U, "dw")   # <= 30001 / 2048 / 32 + 4 + 2048 / 8 + 8 terms in turn
     y, s = rms_norm(x, w, 1e-6, residual=r)
     assert torch.equal(torch.autograd.grad(s, x, gy)[0], gy)

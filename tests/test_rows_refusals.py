@@ -34,7 +34,7 @@ def test_c_entries_refuse_bad_arguments():
     assert fwd(rows=0) == 0
     quant = lambda code=1, F=64, group=64: L.iso_rms_norm_quant(0, code, 1, F, group, one, F, None, 0, None, 0, 1e-6, None, None, None, None)
     assert "code" in _message(quant(code=3)) and "group" in _message(quant(group=16)) and "group" in _message(quant(F=96, group=64)) and "null" in _message(quant())
-    back = lambda scratch=0, dw=one: L.iso_rms_norm_backward(0, 8, 4, one, 4, None, 0, one, one, 4, None, 0, None, dw, one, scratch, None)
+    back = lambda scratch=0, dw=one: L.iso_rms_norm_backward(0, 8, 4, one, 4, None, 0, None, 0, one, one, 4, None, 0, None, dw, one, scratch, None)
     assert "scratch" in _message(back()) and "null" in _message(back(dw=None))
     assert L.iso_rms_norm_scratch_bytes(0, 8, 4) > 0 and L.iso_rms_norm_scratch_bytes(0, 0, 4) == 0
     write = lambda n=2, P=4, first=0, index=None, owner=None: L.iso_rows8_write(0, 1, n, 4, 4, P, one, 4, first, index, 1, owner, one, one, None)
