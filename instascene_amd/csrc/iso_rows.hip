@@ -9,7 +9,9 @@
 // All of it is bound by memory: every element is read once, kept in registers between the reduction and the output, and
 // written once.  `tpr` threads (a power of two) share a row, NV vectors of 16 input bytes each, vector j = t + k tpr, so
 // that a wave's loads are contiguous; rows longer than the registers hold are read a second time (the *_long kernels).
-// Sums of squares are held in 64 bits (two instructions per element, hidden behind the loads): no overflow for any finite row.
+// Sums of squares are held in 32 bits, in short chains (a vector's elements side by side, then a tree); a row whose sum leaves
+// [1e-30, 1e37] is summed again in 64 bits, so that no finite row overflows or vanishes.  (64 bits throughout cost a quarter of the time of
+// narrow rows: conversions and 64-bit additions run at a fraction of the rate.)
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -21,51 +23,75 @@ template <class T> struct RowVec { static constexpr int N = 16 / (int)sizeof(T);
 // (alignment of one element: rows of odd widths and views of buckets start anywhere; gfx950 loads unaligned vectors)
 template <class T, int N> struct Unaligned { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
 
-// v[i] = p[i] for i < left, 0 beyond
-template <class T, int N> __device__ __forceinline__ void row_load(const T* p, int left, float (&v)[N]) {
-    if (left >= N) {
-        const typename Unaligned<T, N>::type q = *reinterpret_cast<const typename Unaligned<T, N>::type*>(p);
+// sixteen bytes of a row as they lie in memory, zeros beyond its F elements and for rows that are off.  EVEN: F is a multiple of the
+// vector, so a vector lies in the row or behind it: the address is drawn back into the row and the value dropped, without a branch.
+// NT: past the caches (a stream that is longer than they are and not read again).
+template <class T, int N, bool EVEN, bool NT = false> __device__ __forceinline__ typename Unaligned<T, N>::type raw_load(const T* row, int at, int F, bool on) {
+    typedef typename Unaligned<T, N>::type V;
+    V q = {};
+    if constexpr (EVEN) {
+        const V* p = reinterpret_cast<const V*>(row + min(at, F - N));
+        if constexpr (NT) q = __builtin_nontemporal_load(p);
+        else q = *p;
+        if (!on || at >= F) q = V{};
+    } else if (on) {
+        if (at + N <= F) {
+            const V* p = reinterpret_cast<const V*>(row + at);
+            if constexpr (NT) q = __builtin_nontemporal_load(p);
+            else q = *p;
+        } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = (float)q[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = i < left ? (float)p[i] : 0.0f;
+            for (int i = 0; i < N; i++)
+                if (at + i < F) q[i] = row[at + i];
+        }
     }
+    return q;
+}
+template <class T, int N> __device__ __forceinline__ void raw_float(const typename Unaligned<T, N>::type& q, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = (float)q[i];
+}
+template <class T, int N, bool EVEN> __device__ __forceinline__ void row_load(const T* row, int at, int F, bool on, float (&v)[N]) {
+    raw_float<T, N>(raw_load<T, N, EVEN>(row, at, F, on), v);
 }
 // v = x + res (res may be NULL)
-template <class T, int N> __device__ __forceinline__ void sum_load(const T* x, const T* res, int left, float (&v)[N]) {
-    row_load<T, N>(x, left, v);
+template <class T, int N, bool EVEN> __device__ __forceinline__ void sum_load(const T* x, const T* res, int at, int F, bool on, float (&v)[N]) {
+    row_load<T, N, EVEN>(x, at, F, on, v);
     if (res) {
         float r[N];
-        row_load<T, N>(res, left, r);
+        row_load<T, N, EVEN>(res, at, F, on, r);
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] += r[i];
     }
 }
-template <class T, int N> __device__ __forceinline__ void row_store(T* p, int left, const float (&v)[N]) {
-    if (left >= N) {
-        typename Unaligned<T, N>::type q;
+// row[at + i] = v[i], rounded to nearest even, within the row (at < F)
+template <class T, int N, bool EVEN, bool NT = false> __device__ __forceinline__ void row_store(T* row, int at, int F, const float (&v)[N]) {
+    typedef typename Unaligned<T, N>::type V;
+    if (EVEN || at + N <= F) {
+        V q;
 #pragma unroll
-        for (int i = 0; i < N; i++) q[i] = (T)v[i];          // round to nearest even
-        *reinterpret_cast<typename Unaligned<T, N>::type*>(p) = q;
+        for (int i = 0; i < N; i++) q[i] = (T)v[i];
+        if constexpr (NT) __builtin_nontemporal_store(q, reinterpret_cast<V*>(row + at));
+        else *reinterpret_cast<V*>(row + at) = q;
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++)
-            if (i < left) p[i] = (T)v[i];
+            if (at + i < F) row[at + i] = (T)v[i];
     }
 }
 // the gain: 32 bits or the rows' type; NULL = 1
-template <class T, int N> __device__ __forceinline__ void gain_load(const void* w, int w32, int at, int left, float (&v)[N]) {
+template <class T, int N, bool EVEN> __device__ __forceinline__ void gain_load(const void* w, int w32, int at, int F, float (&v)[N]) {
     if (w == nullptr) {
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = 1.0f;
-    } else if (w32) row_load<float, N>((const float*)w + at, left, v);
-    else row_load<T, N>((const T*)w + at, left, v);
+    } else if (w32) row_load<float, N, EVEN>((const float*)w, at, F, true, v);
+    else row_load<T, N, EVEN>((const T*)w, at, F, true, v);
 }
 
 // ---- sums and maxima over the tpr threads of a row.  Within 16 lanes by DPP (quad_perm, then the mirrors of 8 and 16 lanes: every lane of
 // a half already holds its half's value), across 16 and 32 lanes by the permlane swaps: no trip through LDS.  All lanes of the wave have to
-// be active.  Between waves `lds` has two slots per wave; `turn` alternates between them so that one barrier per reduction is enough.
+// be active.  Between waves (tpr > 64: the workgroup is one row) `lds` has two slots per wave; `turn` alternates between them so that one
+// barrier per reduction is enough.
 template <int CTRL> __device__ __forceinline__ unsigned lane_dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
 // the value of the partner at distance 1, 2, 4, 8 (STEP 0..3; 4 and 8 mirrored), 16, 32
 template <int STEP> __device__ __forceinline__ unsigned lane_partner(unsigned v) {
@@ -79,13 +105,14 @@ template <int STEP> __device__ __forceinline__ unsigned lane_partner(unsigned v)
         return up ? q[0] : q[1];
     }
 }
+template <int STEP> __device__ __forceinline__ float lane_partner(float v) { return __uint_as_float(lane_partner<STEP>(__float_as_uint(v))); }
 template <int STEP> __device__ __forceinline__ double lane_partner(double v) {
     const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
     const unsigned lo = lane_partner<STEP>((unsigned)b), hi = lane_partner<STEP>((unsigned)(b >> 32));
     return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
 // over the lanes of aligned segments of n (a power of two) lanes of a wave
-__device__ __forceinline__ double lanes_sum(double v, int n) {
+template <class S> __device__ __forceinline__ S lanes_sum(S v, int n) {
     if (n > 1) v += lane_partner<0>(v);
     if (n > 2) v += lane_partner<1>(v);
     if (n > 4) v += lane_partner<2>(v);
@@ -103,33 +130,66 @@ __device__ __forceinline__ unsigned lanes_max(unsigned v, int n) {
     if (n > 32) v = max(v, lane_partner<5>(v));
     return v;
 }
-__device__ __forceinline__ double row_sum(double v, int tpr, double (*lds)[16], int turn) {
+__device__ __forceinline__ int row_waves(int tpr) { return tpr >> 6; }
+template <class S> __device__ __forceinline__ S row_sum(S v, int tpr, double (*lds)[16], int turn) {
     v = lanes_sum(v, tpr);
     if (tpr > 64) {
-        const int wave = threadIdx.x >> 6, n = tpr >> 6, first = wave & ~(n - 1);
-        if ((threadIdx.x & 63) == 0) lds[turn][wave] = v;
+        if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = (double)v;          // (exact)
         __syncthreads();
-        v = 0.0;
-        for (int i = 0; i < n; i++) v += lds[turn][first + i];
+        v = (S)0;
+        for (int i = 0; i < row_waves(tpr); i++) v += (S)lds[turn][i];
     }
     return v;
 }
 __device__ __forceinline__ unsigned row_max(unsigned v, int tpr, double (*lds)[16], int turn) {
     v = lanes_max(v, tpr);
     if (tpr > 64) {
-        const int wave = threadIdx.x >> 6, n = tpr >> 6, first = wave & ~(n - 1);
-        if ((threadIdx.x & 63) == 0) lds[turn][wave] = (double)v;          // (exact: 32 bits)
+        if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = (double)v;          // (exact: 32 bits)
         __syncthreads();
         v = 0;
-        for (int i = 0; i < n; i++) v = max(v, (unsigned)lds[turn][first + i]);
+        for (int i = 0; i < row_waves(tpr); i++) v = max(v, (unsigned)lds[turn][i]);
     }
     return v;
 }
-// 1 / sqrt(ss / F + eps); mean squares beyond the range of 32 bits go through 64
-__device__ __forceinline__ float rms_inverse(double ss, double inv_F, float eps) {
-    const double m = ss * inv_F + (double)eps;
-    if (m < 1e37) return 1.0f / __builtin_sqrtf((float)m);
-    return (float)(1.0 / __builtin_sqrt(m));
+// The sum of squares of a row of which this thread holds v[NV][N]; `on`: the row is one (the others may be anything).  Returned as
+// (fast, wide): wide < 0 where the 32-bit sum is good.  The test is the same in all threads of a row; a wave that shares several rows
+// repeats the sum for all of them.
+template <int NV, int N> __device__ __forceinline__ float row_squares(const float (&v)[NV][N], bool on, int tpr, double (*lds)[16], double& wide) {
+    float acc[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) acc[e] = v[0][e] * v[0][e];
+#pragma unroll
+    for (int k = 1; k < NV; k++)
+#pragma unroll
+        for (int e = 0; e < N; e++) acc[e] = __builtin_fmaf(v[k][e], v[k][e], acc[e]);
+#pragma unroll
+    for (int o = N / 2; o >= 1; o >>= 1)
+#pragma unroll
+        for (int e = 0; e < o; e++) acc[e] += acc[e + o];
+    const float ss = row_sum(acc[0], tpr, lds, 0);
+    const bool odd = on && !(ss > 1e-30f && ss < 1e37f);
+    wide = -1.0;
+    if (__any(odd)) {           // (tpr > 64: one row, all of its waves agree)
+        double s = 0.0;
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int e = 0; e < N; e++) s += (double)v[k][e] * (double)v[k][e];
+        if (tpr > 64) __syncthreads();          // slot 0 has been read by everybody
+        s = row_sum(s, tpr, lds, 0);
+        if (odd) wide = s;
+    }
+    return ss;
+}
+// 1 / sqrt(ss / F + eps): v_rsq_f32 is within one step
+__device__ __forceinline__ float rms_inverse(float ss, double wide, double inv_F, float eps) {
+    if (__builtin_expect(wide >= 0.0 || wide != wide, 0)) return (float)(1.0 / __builtin_sqrt(wide * inv_F + (double)eps));
+    return __builtin_amdgcn_rsqf(__builtin_fmaf(ss, (float)inv_F, eps));
+}
+// 1 / (sqrt(ss) + eps): v_sqrt_f32 and v_rcp_f32 are within one step
+__device__ __forceinline__ float l2_inverse(float ss, double wide, float eps) {
+    if (__builtin_expect(wide >= 0.0 || wide != wide, 0)) return (float)(1.0 / (__builtin_sqrt(wide) + (double)eps));
+    return __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(ss) + eps);
 }
 
 // ---- 8-bit codes -----------------------------------------------------------------------------------------------------------------
@@ -203,13 +263,25 @@ template <int CODE> __device__ __forceinline__ unsigned encode4(const float* t, 
     }
     return in;
 }
-template <int N> __device__ __forceinline__ void code_store(unsigned char* p, int left, const unsigned (&c)[N / 4]) {
-    if (left >= N) __builtin_memcpy(p, c, N);
-    else {
+template <int N, bool EVEN> __device__ __forceinline__ void code_store(unsigned char* row, int at, int F, const unsigned (&c)[N / 4], int nt) {
+    typedef unsigned V __attribute__((ext_vector_type(N / 4), aligned(1)));
+    if (EVEN || at + N <= F) {
+        V q;
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) q[i] = c[i];
+        if (nt) __builtin_nontemporal_store(q, reinterpret_cast<V*>(row + at));
+        else *reinterpret_cast<V*>(row + at) = q;
+    } else {
 #pragma unroll
         for (int i = 0; i < N; i++)
-            if (i < left) p[i] = (unsigned char)(c[i / 4] >> (8 * (i & 3)));
+            if (at + i < F) row[at + i] = (unsigned char)(c[i / 4] >> (8 * (i & 3)));
     }
+}
+template <int N> __device__ __forceinline__ unsigned top_bits_of(const float (&v)[N]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+    return m;
 }
 
 // ---- where a written row goes ----------------------------------------------------------------------------------------------------
@@ -256,6 +328,7 @@ struct RmsArgs {
     long long rows, row0;   // this launch starts at row row0
     int F, tpr, tsh, norm, w32;     // tpr = 1 << tsh threads per row
     int groups, gshift;     // groups per row and log2 of their columns; one group: 1 and 31
+    int nt;                 // codes past the caches
     float eps;
     double inv_F;
     const void* x;
@@ -270,7 +343,7 @@ struct RmsArgs {
     float* scales;          // [P, groups]
     RowTarget to;
 };
-template <class T, int NV, int OUT> __global__ __launch_bounds__(512) void rms_forward_kernel(RmsArgs a) {
+template <class T, int NV, int OUT, bool EVEN> __global__ __launch_bounds__(512) void rms_forward_kernel(RmsArgs a) {
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1);
@@ -279,63 +352,45 @@ template <class T, int NV, int OUT> __global__ __launch_bounds__(512) void rms_f
     const T* x = (const T*)a.x + (on ? i : 0) * a.ldx;
     const T* res = a.res ? (const T*)a.res + (on ? i : 0) * a.ldr : nullptr;
     float v[NV][N];
-    double ss = 0.0;
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-        const int at = (t + k * tpr) * N, left = on ? a.F - at : 0;
-        if (left <= 0) {
-#pragma unroll
-            for (int e = 0; e < N; e++) v[k][e] = 0.0f;
-            continue;
-        }
-        sum_load<T, N>(x + at, res ? res + at : nullptr, left, v[k]);
-    }
+    for (int k = 0; k < NV; k++) sum_load<T, N, EVEN>(x, res, (t + k * tpr) * N, a.F, on, v[k]);
+    float rstd = 1.0f;
     if (a.norm) {
-#pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int e = 0; e < N; e++) ss += (double)v[k][e] * (double)v[k][e];
-        ss = row_sum(ss, tpr, lds, 0);
+        double wide;
+        const float ss = row_squares(v, on, tpr, lds, wide);
+        rstd = rms_inverse(ss, wide, a.inv_F, a.eps);
     }
-    const float rstd = a.norm ? rms_inverse(ss, a.inv_F, a.eps) : 1.0f;
     if (a.rstd && on && t == 0) a.rstd[i] = rstd;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        const int at = (t + k * tpr) * N, left = on ? a.F - at : 0;
-        if (left <= 0) continue;
-        if (a.s) row_store<T, N>((T*)a.s + i * a.F + at, left, v[k]);
+        const int at = (t + k * tpr) * N;
+        if (at >= a.F || !on) continue;
+        if (a.s) row_store<T, N, EVEN>((T*)a.s + i * a.F, at, a.F, v[k]);
         float w[N];
-        gain_load<T, N>(a.w, a.w32, at, left, w);
+        gain_load<T, N, EVEN>(a.w, a.w32, at, a.F, w);
 #pragma unroll
         for (int e = 0; e < N; e++) v[k][e] = OUT == 0 ? v[k][e] * rstd * w[e] : v[k][e] * w[e];
-        if (OUT == 0) row_store<T, N>((T*)a.y + i * a.F + at, left, v[k]);
+        if constexpr (OUT == 0) row_store<T, N, EVEN>((T*)a.y + i * a.F, at, a.F, v[k]);
     }
     if constexpr (OUT != 0) {
         const long long row = row_target(a.to, i, a.rows, t, tpr, lds);
         const int seg = a.groups == 1 ? 0 : (1 << a.gshift) / N;
-        unsigned top_bits = 0;
+        unsigned top = 0;
         if (seg == 0) {
 #pragma unroll
-            for (int k = 0; k < NV; k++)
-#pragma unroll
-                for (int e = 0; e < N; e++) top_bits = max(top_bits, __float_as_uint(v[k][e]) & 0x7fffffffu);
-            top_bits = row_max(top_bits, tpr, lds, 1);
+            for (int k = 0; k < NV; k++) top = max(top, top_bits_of(v[k]));
+            top = row_max(top, tpr, lds, 1);
         }
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int at = (t + k * tpr) * N, left = a.F - at;
-            if (seg != 0) {             // a group's vectors lie in `seg` neighbouring lanes of one wave
-                top_bits = 0;
-#pragma unroll
-                for (int e = 0; e < N; e++) top_bits = max(top_bits, __float_as_uint(v[k][e]) & 0x7fffffffu);
-                top_bits = lanes_max(top_bits, seg);
-            }
-            const Group8 g = group_scale<OUT>(top_bits);
-            if (row < 0 || left <= 0) continue;
+            const int at = (t + k * tpr) * N;
+            if (seg != 0) top = lanes_max(top_bits_of(v[k]), seg);          // a group's vectors lie in `seg` neighbouring lanes of one wave
+            const Group8 g = group_scale<OUT>(top);
+            if (row < 0 || at >= a.F) continue;
             unsigned c[N / 4];
 #pragma unroll
             for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[k][4 * q], g);
-            code_store<N>(a.codes + row * a.F + at, left, c);
+            code_store<N, EVEN>(a.codes + row * a.F, at, a.F, c, a.nt);
             if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
         }
     }
@@ -350,54 +405,47 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
     const T* x = (const T*)a.x + i * a.ldx;
     const T* res = a.res ? (const T*)a.res + i * a.ldr : nullptr;
     const long long row = OUT != 0 ? row_target(a.to, i, a.rows, t, tpr, lds) : i;
+    const bool by_row = OUT != 0 && a.groups == 1;
     double ss = 0.0;
     unsigned row_top = 0;
-    const bool by_row = OUT != 0 && a.groups == 1;
     for (int at = t * N; at < a.F; at += tpr * N) {
         float v[N], w[N];
-        sum_load<T, N>(x + at, res ? res + at : nullptr, a.F - at, v);
+        sum_load<T, N, false>(x, res, at, a.F, true, v);
 #pragma unroll
         for (int e = 0; e < N; e++) ss += (double)v[e] * (double)v[e];
         if (by_row) {
-            gain_load<T, N>(a.w, a.w32, at, a.F - at, w);
+            gain_load<T, N, false>(a.w, a.w32, at, a.F, w);
 #pragma unroll
-            for (int e = 0; e < N; e++) row_top = max(row_top, __float_as_uint(v[e] * w[e]) & 0x7fffffffu);
+            for (int e = 0; e < N; e++) v[e] *= w[e];
+            row_top = max(row_top, top_bits_of(v));
         }
     }
     float rstd = 1.0f;
-    if (a.norm) rstd = rms_inverse(row_sum(ss, tpr, lds, 0), a.inv_F, a.eps);
+    if (a.norm) rstd = rms_inverse(0.0f, row_sum(ss, tpr, lds, 0), a.inv_F, a.eps);
     if (by_row) row_top = row_max(row_top, tpr, lds, 1);
     if (a.rstd && t == 0) a.rstd[i] = rstd;
     const int seg = OUT == 0 || by_row ? 0 : (1 << a.gshift) / N;
-    // (all threads of a wave take every step together: the groups' maxima are shuffled)
+    // (all threads of a wave take every step together: the groups' maxima go from lane to lane)
     for (int base = 0; base < a.F; base += tpr * N) {
-        const int at = base + t * N, left = a.F - at;
+        const int at = base + t * N;
+        const bool in = at < a.F;
         float v[N], w[N];
-        sum_load<T, N>(x + at, res ? res + at : nullptr, left, v);          // (left <= 0: nothing is read)
-        if (a.s && left > 0) row_store<T, N>((T*)a.s + i * a.F + at, left, v);
-        if (left > 0) gain_load<T, N>(a.w, a.w32, at, left, w);
-        else {
+        sum_load<T, N, false>(x, res, at, a.F, in, v);
+        if (a.s && in) row_store<T, N, false>((T*)a.s + i * a.F, at, a.F, v);
 #pragma unroll
-            for (int e = 0; e < N; e++) w[e] = 0.0f;
-        }
+        for (int e = 0; e < N; e++) w[e] = 0.0f;
+        if (in) gain_load<T, N, false>(a.w, a.w32, at, a.F, w);
 #pragma unroll
         for (int e = 0; e < N; e++) v[e] = OUT == 0 ? v[e] * rstd * w[e] : v[e] * w[e];
         if constexpr (OUT == 0) {
-            if (left > 0) row_store<T, N>((T*)a.y + i * a.F + at, left, v);
+            if (in) row_store<T, N, false>((T*)a.y + i * a.F, at, a.F, v);
         } else {
-            unsigned top_bits = row_top;
-            if (seg != 0) {
-                top_bits = 0;
-#pragma unroll
-                for (int e = 0; e < N; e++) top_bits = max(top_bits, __float_as_uint(v[e]) & 0x7fffffffu);
-                top_bits = lanes_max(top_bits, seg);
-            }
-            const Group8 g = group_scale<OUT>(top_bits);
-            if (row >= 0 && left > 0) {
+            const Group8 g = group_scale<OUT>(seg != 0 ? lanes_max(top_bits_of(v), seg) : row_top);
+            if (row >= 0 && in) {
                 unsigned c[N / 4];
 #pragma unroll
                 for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[4 * q], g);
-                code_store<N>(a.codes + row * a.F + at, left, c);
+                code_store<N, false>(a.codes + row * a.F, at, a.F, c, a.nt);
                 if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
             }
         }
@@ -421,93 +469,112 @@ struct RmsBackArgs {
     void* ds;               // or NULL: [rows, F]
     float* dw_part;         // or NULL: [gridDim.x, F]
 };
-template <class T, int NV> __global__ __launch_bounds__(512) void rms_backward_kernel(RmsBackArgs a) {
+template <class T, int NV, bool EVEN, bool NT> __global__ __launch_bounds__(512) void rms_backward_kernel(RmsBackArgs a) {
     constexpr int N = RowVec<T>::N;
+    typedef typename Unaligned<T, N>::type V;
     __shared__ double lds[2][16];
-    __shared__ float part[8][64 * N];       // the waves' sums of one vector slot
+    __shared__ float part[4][64 * N];       // the waves' sums of one vector slot
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), rpb = blockDim.x >> a.tsh;
     float dw[NV][N], w[NV][N];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        const int at = (t + k * tpr) * N, left = a.F - at;
+        const int at = (t + k * tpr) * N;
 #pragma unroll
         for (int e = 0; e < N; e++) { dw[k][e] = 0.0f; w[k][e] = 0.0f; }
-        if (left > 0) gain_load<T, N>(a.w, a.w32, at, left, w[k]);
+        if (at < a.F) gain_load<T, N, EVEN>(a.w, a.w32, at, a.F, w[k]);
     }
-    int turn = 0;
-    for (long long r0 = (long long)blockIdx.x * rpb; r0 < a.rows; r0 += (long long)gridDim.x * rpb, turn ^= 1) {
-        const long long i = r0 + (threadIdx.x >> a.tsh);
-        const bool on = i < a.rows;
-        const float rstd = on ? a.rstd[i] : 0.0f;
-        const T* x = (const T*)a.x + (on ? i : 0) * a.ldx;
-        const T* res = a.res ? (const T*)a.res + (on ? i : 0) * a.ldr : nullptr;
-        const T* gy = (const T*)a.gy + (on ? i : 0) * a.ldg;
-        float h[NV][N], g[NV][N];
-        float c = 0.0f;
+    const long long step = (long long)gridDim.x * rpb;
+    long long i = (long long)blockIdx.x * rpb + (threadIdx.x >> a.tsh);
+    V xq[NV], rq[NV], gq[NV], sq[NV];
+    float rstd;
+    auto fetch = [&](long long row) {           // (rows beyond the last: zeros)
+        const bool on = row < a.rows;
+        const long long r = on ? row : 0;
+        rstd = on ? a.rstd[r] : 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int at = (t + k * tpr) * N, left = on ? a.F - at : 0;
-#pragma unroll
-            for (int e = 0; e < N; e++) { h[k][e] = 0.0f; g[k][e] = 0.0f; }
-            if (left <= 0) continue;
-            sum_load<T, N>(x + at, res ? res + at : nullptr, left, h[k]);
-            row_load<T, N>(gy + at, left, g[k]);
+            const int at = (t + k * tpr) * N;
+            xq[k] = raw_load<T, N, EVEN, NT>((const T*)a.x + r * a.ldx, at, a.F, on);
+            gq[k] = raw_load<T, N, EVEN, NT>((const T*)a.gy + r * a.ldg, at, a.F, on);
+            if (a.res) rq[k] = raw_load<T, N, EVEN, NT>((const T*)a.res + r * a.ldr, at, a.F, on);
+            if (a.gs) sq[k] = raw_load<T, N, EVEN, NT>((const T*)a.gs + r * a.ldgs, at, a.F, on);
         }
+    };
+    fetch(i);
+    int turn = 0;
+    for (long long r0 = (long long)blockIdx.x * rpb; r0 < a.rows; r0 += step, i += step, turn ^= 1) {
+        const bool on = i < a.rows;
+        const float rs = rstd;
+        float h[NV][N], g[NV][N], c[N];
+        V q[NV];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            raw_float<T, N>(xq[k], h[k]);
+            raw_float<T, N>(gq[k], g[k]);
+            if (a.gs) q[k] = sq[k];
+            if (a.res) {
+                float r[N];
+                raw_float<T, N>(rq[k], r);
+#pragma unroll
+                for (int e = 0; e < N; e++) h[k][e] += r[e];
+            }
+        }
+        fetch(i + step);                        // in flight while this row is reduced and written
+#pragma unroll
+        for (int e = 0; e < N; e++) c[e] = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
             for (int e = 0; e < N; e++) {
-                h[k][e] *= rstd;
-                dw[k][e] += g[k][e] * h[k][e];
+                h[k][e] *= rs;
+                dw[k][e] = __builtin_fmaf(g[k][e], h[k][e], dw[k][e]);
                 g[k][e] *= w[k][e];
-                c += g[k][e] * h[k][e];
+                c[e] = __builtin_fmaf(g[k][e], h[k][e], c[e]);
             }
-        const float mean = (float)row_sum((double)c, tpr, lds, turn) / (float)a.F;
+#pragma unroll
+        for (int o = N / 2; o >= 1; o >>= 1)
+#pragma unroll
+            for (int e = 0; e < o; e++) c[e] += c[e + o];
+        const float mean = row_sum(c[0], tpr, lds, turn) / (float)a.F;
         if (a.ds == nullptr) continue;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            const int at = (t + k * tpr) * N, left = on ? a.F - at : 0;
-            if (left <= 0) continue;
+            const int at = (t + k * tpr) * N;
+            if (at >= a.F || !on) continue;
             float d[N];
 #pragma unroll
-            for (int e = 0; e < N; e++) d[e] = rstd * (g[k][e] - h[k][e] * mean);
+            for (int e = 0; e < N; e++) d[e] = rs * (g[k][e] - h[k][e] * mean);
             if (a.gs) {
-                float q[N];
-                row_load<T, N>((const T*)a.gs + i * a.ldgs + at, left, q);
+                float u[N];
+                raw_float<T, N>(q[k], u);
 #pragma unroll
-                for (int e = 0; e < N; e++) d[e] += q[e];
+                for (int e = 0; e < N; e++) d[e] += u[e];
             }
-            row_store<T, N>((T*)a.ds + i * a.F + at, left, d);
+            row_store<T, N, EVEN, NT>((T*)a.ds + i * a.F, at, a.F, d);
         }
     }
     if (a.dw_part == nullptr) return;
     // the rows of a wave first, then the waves, in a fixed order
-    const int lanes = min(tpr, 64);
+    float* out = a.dw_part + (long long)blockIdx.x * a.F;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        for (int o = 32; o >= lanes; o >>= 1)
+        for (int o = 32; o >= tpr; o >>= 1)
 #pragma unroll
             for (int e = 0; e < N; e++) dw[k][e] += __shfl_xor(dw[k][e], o);
         const int at = (t + k * tpr) * N;
-        if (rpb == 1) {
-            if (at < a.F) row_store<float, N>(a.dw_part + (long long)blockIdx.x * a.F + at, a.F - at, dw[k]);
-            continue;
+        if (rpb > 1) {                          // (tpr <= 64: every wave has sums of the same columns)
+            const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+            __syncthreads();
+            if (lane < tpr)
+#pragma unroll
+                for (int e = 0; e < N; e++) part[wave][lane * N + e] = dw[k][e];
+            __syncthreads();
+            if (threadIdx.x < tpr)
+                for (int q = 1; q < (int)(blockDim.x >> 6); q++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) dw[k][e] += part[q][lane * N + e];
         }
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, per_row = max(1, tpr >> 6), n = (int)(blockDim.x >> 6) / per_row;
-        __syncthreads();
-        if (lane < lanes)
-#pragma unroll
-            for (int e = 0; e < N; e++) part[wave][lane * N + e] = dw[k][e];
-        __syncthreads();
-        if (threadIdx.x < tpr && at < a.F) {
-            float sum[N];
-#pragma unroll
-            for (int e = 0; e < N; e++) sum[e] = 0.0f;
-            for (int q = 0; q < n; q++)
-#pragma unroll
-                for (int e = 0; e < N; e++) sum[e] += part[q * per_row + wave][lane * N + e];
-            row_store<float, N>(a.dw_part + (long long)blockIdx.x * a.F + at, a.F - at, sum);
-        }
+        if (threadIdx.x < tpr && at < a.F) row_store<float, N, EVEN>(out, at, a.F, dw[k]);
     }
 }
 // rows beyond the registers: ds by one workgroup per row (read twice), dw by columns
@@ -523,30 +590,29 @@ template <class T> __global__ __launch_bounds__(512) void rms_backward_long_kern
     double c = 0.0;
     for (int at = t * N; at < a.F; at += tpr * N) {
         float h[N], g[N], w[N];
-        sum_load<T, N>(x + at, res ? res + at : nullptr, a.F - at, h);
-        row_load<T, N>(gy + at, a.F - at, g);
-        gain_load<T, N>(a.w, a.w32, at, a.F - at, w);
+        sum_load<T, N, false>(x, res, at, a.F, true, h);
+        row_load<T, N, false>(gy, at, a.F, true, g);
+        gain_load<T, N, false>(a.w, a.w32, at, a.F, w);
         float p = 0.0f;
 #pragma unroll
-        for (int e = 0; e < N; e++)
-            if (at + e < a.F) p += g[e] * w[e] * (h[e] * rstd);
+        for (int e = 0; e < N; e++) p += g[e] * w[e] * (h[e] * rstd);
         c += (double)p;
     }
     const float mean = (float)row_sum(c, tpr, lds, 0) / (float)a.F;
     for (int at = t * N; at < a.F; at += tpr * N) {
         float h[N], g[N], w[N], d[N];
-        sum_load<T, N>(x + at, res ? res + at : nullptr, a.F - at, h);
-        row_load<T, N>(gy + at, a.F - at, g);
-        gain_load<T, N>(a.w, a.w32, at, a.F - at, w);
+        sum_load<T, N, false>(x, res, at, a.F, true, h);
+        row_load<T, N, false>(gy, at, a.F, true, g);
+        gain_load<T, N, false>(a.w, a.w32, at, a.F, w);
 #pragma unroll
         for (int e = 0; e < N; e++) d[e] = rstd * (g[e] * w[e] - h[e] * rstd * mean);
         if (a.gs) {
             float q[N];
-            row_load<T, N>((const T*)a.gs + i * a.ldgs + at, a.F - at, q);
+            row_load<T, N, false>((const T*)a.gs + i * a.ldgs, at, a.F, true, q);
 #pragma unroll
             for (int e = 0; e < N; e++) d[e] += q[e];
         }
-        row_store<T, N>((T*)a.ds + i * a.F + at, a.F - at, d);
+        row_store<T, N, false>((T*)a.ds + i * a.F, at, a.F, d);
     }
 }
 template <class T> __global__ __launch_bounds__(256) void rms_dw_columns_kernel(RmsBackArgs a, int slices) {
@@ -594,90 +660,75 @@ struct ReadArgs {
     const void* index;      // or NULL
     void* out;              // [rows, F]
 };
-template <int CODE, int N> __device__ __forceinline__ void code_load(const unsigned char* p, int left, float (&v)[N]) {
-    if (left >= N) {
-        unsigned c[N / 4];
-        __builtin_memcpy(c, p, N);
-#pragma unroll
-        for (int q = 0; q < N / 4; q++) Code8<CODE>::unpack4(c[q], v + 4 * q);
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; e++) v[e] = e < left ? Code8<CODE>::one(p[e]) : 0.0f;
+// the codes of N columns and their scale as values, zeros beyond the row and for rows that are off
+template <int CODE, int N, bool EVEN> __device__ __forceinline__ void code_load(const ReadArgs& a, long long row, int at, float (&v)[N]) {
+    const unsigned char* codes = a.codes + (row >= 0 ? row : 0) * a.F;
+    const bool in = row >= 0 && at < a.F;
+    const int p = EVEN ? min(at, a.F - N) : at;
+    float scale = 0.0f;
+    unsigned c[N / 4] = {};
+    if (a.P > 0) {          // (an empty table has nothing to draw the address back to)
+        if (EVEN || in) scale = a.scales[(row >= 0 ? row : 0) * a.groups + (p >> a.gshift)];
+        if (EVEN || (in && at + N <= a.F)) __builtin_memcpy(c, codes + p, N);
+        else if (in)
+            for (int e = 0; e < N && at + e < a.F; e++) c[e / 4] |= (unsigned)codes[at + e] << (8 * (e & 3));
     }
+#pragma unroll
+    for (int q = 0; q < N / 4; q++) Code8<CODE>::unpack4(c[q], v + 4 * q);
+#pragma unroll
+    for (int e = 0; e < N; e++) v[e] = in && (EVEN || at + e < a.F) ? v[e] * scale : 0.0f;
 }
-__device__ __forceinline__ float l2_inverse(double ss, float eps) {
-    const float n = ss < 1e37 ? __builtin_sqrtf((float)ss) : (float)__builtin_sqrt(ss);
-    return 1.0f / (n + eps);
+__device__ __forceinline__ long long read_row(const ReadArgs& a, long long i) {
+    const long long row = a.index == nullptr ? a.first + i : a.is64 ? ((const long long*)a.index)[i] : (long long)((const int*)a.index)[i];
+    return row < a.P ? row : -1;
 }
-template <class T, int CODE, int NV> __global__ __launch_bounds__(512) void rows_read_kernel(ReadArgs a) {
+template <class T, int CODE, int NV, bool EVEN> __global__ __launch_bounds__(512) void rows_read_kernel(ReadArgs a) {
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1);
     const long long i = a.row0 + (long long)blockIdx.x * (blockDim.x >> a.tsh) + (threadIdx.x >> a.tsh);
-    long long row = -1;
-    if (i < a.rows) row = a.index == nullptr ? a.first + i : a.is64 ? ((const long long*)a.index)[i] : (long long)((const int*)a.index)[i];
-    if (row >= a.P) row = -1;
+    const long long row = i < a.rows ? read_row(a, i) : -1;
     float v[NV][N];
-    double ss = 0.0;
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-        const int at = (t + k * tpr) * N, left = row >= 0 ? a.F - at : 0;
-#pragma unroll
-        for (int e = 0; e < N; e++) v[k][e] = 0.0f;
-        if (left <= 0) continue;
-        code_load<CODE, N>(a.codes + row * a.F + at, left, v[k]);
-        const float scale = a.scales[row * a.groups + (at >> a.gshift)];
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-            v[k][e] = e < left ? v[k][e] * scale : 0.0f;
-            ss += (double)v[k][e] * (double)v[k][e];
-        }
-    }
+    for (int k = 0; k < NV; k++) code_load<CODE, N, EVEN>(a, row, (t + k * tpr) * N, v[k]);
     float inv = 1.0f;
-    if (a.norm) inv = l2_inverse(row_sum(ss, tpr, lds, 0), a.eps);
-    if (row < 0) inv = 0.0f;
+    if (a.norm) {
+        double wide;
+        const float ss = row_squares(v, row >= 0, tpr, lds, wide);
+        inv = row >= 0 ? l2_inverse(ss, wide, a.eps) : 0.0f;
+    }
     if (i >= a.rows) return;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        const int at = (t + k * tpr) * N, left = a.F - at;
-        if (left <= 0) continue;
+        const int at = (t + k * tpr) * N;
 #pragma unroll
         for (int e = 0; e < N; e++) v[k][e] *= inv;
-        row_store<T, N>((T*)a.out + i * a.F + at, left, v[k]);
+        if (at < a.F) row_store<T, N, EVEN>((T*)a.out + i * a.F, at, a.F, v[k]);
     }
 }
 template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_long_kernel(ReadArgs a) {
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x;
-    const long long i = a.row0 + blockIdx.x;
-    long long row = a.index == nullptr ? a.first + i : a.is64 ? ((const long long*)a.index)[i] : (long long)((const int*)a.index)[i];
-    if (row >= a.P) row = -1;
+    const long long i = a.row0 + blockIdx.x, row = read_row(a, i);
     float inv = 1.0f;
     if (a.norm) {
         double ss = 0.0;
-        if (row >= 0)
-            for (int at = t * N; at < a.F; at += tpr * N) {
-                float v[N];
-                code_load<CODE, N>(a.codes + row * a.F + at, a.F - at, v);
-                const float scale = a.scales[row * a.groups + (at >> a.gshift)];
+        for (int at = t * N; at < a.F; at += tpr * N) {
+            float v[N];
+            code_load<CODE, N, false>(a, row, at, v);
 #pragma unroll
-                for (int e = 0; e < N; e++)
-                    if (at + e < a.F) ss += (double)(v[e] * scale) * (double)(v[e] * scale);
-            }
-        inv = l2_inverse(row_sum(ss, tpr, lds, 0), a.eps);
+            for (int e = 0; e < N; e++) ss += (double)v[e] * (double)v[e];
+        }
+        ss = row_sum(ss, tpr, lds, 0);
+        inv = row >= 0 ? l2_inverse(0.0f, ss, a.eps) : 0.0f;
     }
     for (int at = t * N; at < a.F; at += tpr * N) {
         float v[N];
+        code_load<CODE, N, false>(a, row, at, v);
 #pragma unroll
-        for (int e = 0; e < N; e++) v[e] = 0.0f;
-        if (row >= 0) {
-            code_load<CODE, N>(a.codes + row * a.F + at, a.F - at, v);
-            const float scale = a.scales[row * a.groups + (at >> a.gshift)];
-#pragma unroll
-            for (int e = 0; e < N; e++) v[e] = v[e] * scale * inv;
-        }
-        row_store<T, N>((T*)a.out + i * a.F + at, a.F - at, v);
+        for (int e = 0; e < N; e++) v[e] *= inv;
+        row_store<T, N, false>((T*)a.out + i * a.F, at, a.F, v);
     }
 }
 

@@ -19,35 +19,56 @@ bool code_type(int c) { return c == iso::CODE_INT8 || c == iso::CODE_E4M3; }
 bool group_ok(int F, int group) { return group == F || ((group == 32 || group == 64 || group == 128) && F % group == 0); }
 int group_shift(int F, int group) { return group == F ? 31 : group == 32 ? 5 : group == 64 ? 6 : 7; }
 
+#ifndef ROWS_GRID
+#define ROWS_GRID 512
+#endif
+#ifndef ROWS_LEAST_FWD
+#define ROWS_LEAST_FWD 1
+#endif
+#ifndef ROWS_LEAST_Q
+#define ROWS_LEAST_Q 2
+#endif
+#ifndef ROWS_LEAST_READ
+#define ROWS_LEAST_READ 2
+#endif
+#ifndef ROWS_NT_BYTES
+#define ROWS_NT_BYTES (128ll << 20)
+#endif
 // threads per row (1 << tsh) and vectors per thread for a row of `vecs` vectors; 0 vectors per thread: the *_long form.
-// A wave and fewer as long as 4 vectors per thread do (no barrier between waves), `least` vectors per thread where the row has them and there
-// are rows enough to fill the chip; where the chip would stand idle, or beyond 4 vectors in a wave, up to 512 threads.
+// Within a wave `least` vectors per thread where there are rows enough to fill the chip all the same (what is done once per row weighs less);
+// beyond a wave 2 per thread; where there are so few rows that the chip would stand idle, up to 512 threads.
 void row_shape(int vecs, long long rows, int least, int max_nv, int& tsh, int& nv) {
     tsh = 0;
     while ((1 << tsh) < vecs && tsh < 6) tsh++;
-    while (tsh > 0 && (1 << tsh) * least > vecs && (1 << (tsh - 1)) * least >= vecs && (rows << (tsh - 1)) >= 2048 * 256) tsh--;
-    while (tsh < 9 && (1 << tsh) < vecs && ((vecs + (1 << tsh) - 1) >> tsh > 4 || (rows << tsh) < 256 * 256)) tsh++;
+    while (tsh > 0 && (vecs + (1 << (tsh - 1)) - 1) >> (tsh - 1) <= least && (rows << (tsh - 1)) >= 2048 * 256) tsh--;
+    while (tsh >= 6 && tsh < 9 && (1 << tsh) < vecs && ((vecs + (1 << tsh) - 1) >> tsh > 2 || (rows << tsh) < 256 * 256)) tsh++;
     const int need = (vecs + (1 << tsh) - 1) >> tsh;
     nv = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : need <= 8 ? 8 : 0;
     if (nv > max_nv) nv = 0;
     if (nv == 0) tsh = 9;
 }
+int row_block(int tsh) { return tsh > 6 ? 1 << tsh : 256; }         // beyond a wave a workgroup is one row
 
-#define ROWS_NV(nv, call_nv, call_long) \
-    do { if (nv == 1) { call_nv(1); } else if (nv == 2) { call_nv(2); } else if (nv == 4) { call_nv(4); } else if (nv == 8) { call_nv(8); } else { call_long; } } while (0)
+#define ROWS_NV(nv, even, call, call_long) \
+    do { if (nv == 1) { if (even) { call(1, true); } else { call(1, false); } } else if (nv == 2) { if (even) { call(2, true); } else { call(2, false); } } \
+         else if (nv == 4) { if (even) { call(4, true); } else { call(4, false); } } else if (nv == 8) { if (even) { call(8, true); } else { call(8, false); } } \
+         else { call_long; } } while (0)
 
 template <class T, int OUT> void launch_forward(iso::RmsArgs a, hipStream_t s) {
+    constexpr int N = iso::RowVec<T>::N;
     int nv;
-    row_shape((a.F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, a.rows, OUT == 0 ? 1 : 2, 8, a.tsh, nv);
+    row_shape((a.F + N - 1) / N, a.rows, OUT == 0 ? ROWS_LEAST_FWD : ROWS_LEAST_Q, 8, a.tsh, nv);
     a.tpr = 1 << a.tsh;
-    const int block = std::max(256, a.tpr);
-    const long long step = MAX_THREADS / block * (block / a.tpr);
+    a.nt = a.rows * a.F * (long long)sizeof(T) >= ROWS_NT_BYTES;
+    const bool even = a.F % N == 0;
+    const int block = row_block(a.tsh), rpb = block >> a.tsh;
+    const long long step = MAX_THREADS / block * rpb;
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
-        const dim3 grid((unsigned)((n + block / a.tpr - 1) / (block / a.tpr)));
-#define FWD(NV) hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT>), grid, dim3(block), 0, s, a)
-#define FWD_LONG hipLaunchKernelGGL((iso::rms_forward_long_kernel<T, OUT>), dim3((unsigned)n), dim3(512), 0, s, a)
-        ROWS_NV(nv, FWD, FWD_LONG);
+        const dim3 grid((unsigned)((n + rpb - 1) / rpb));
+#define FWD(NV, EVEN) hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, EVEN>), grid, dim3(block), 0, s, a)
+#define FWD_LONG hipLaunchKernelGGL((iso::rms_forward_long_kernel<T, OUT>), grid, dim3(block), 0, s, a)
+        ROWS_NV(nv, even, FWD, FWD_LONG);
 #undef FWD
 #undef FWD_LONG
     }
@@ -65,11 +86,11 @@ void launch_codes(int code, int type, const iso::RmsArgs& a, hipStream_t s) {
 // workgroups of the backward pass = partial rows of dw: enough to fill the chip, few enough that the partials stay small against the rows
 template <class T> void backward_shape(long long rows, int F, int& tsh, int& nv, int& block, int& grid) {
     row_shape((F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, rows, 1, 4, tsh, nv);
-    const int tpr = 1 << tsh;
-    block = std::max(256, tpr);
+    block = row_block(tsh);
     if (nv == 0) { grid = (int)std::min<long long>(64, std::max<long long>(1, rows)); return; }       // slices of the columns' sums
-    const long long need = (rows + block / tpr - 1) / (block / tpr);
-    const long long most = std::max<long long>(512, std::min<long long>(2048, (1 << 20) / F));
+    const int rpb = block >> tsh;
+    const long long need = (rows + rpb - 1) / rpb;
+    const long long most = std::max<long long>(ROWS_GRID, std::min<long long>(2048, (1 << 20) / F));
     grid = (int)std::max<long long>(1, std::min(need, most));
 }
 void backward_shape_type(int type, long long rows, int F, int& tsh, int& nv, int& block, int& grid) {
@@ -77,29 +98,39 @@ void backward_shape_type(int type, long long rows, int F, int& tsh, int& nv, int
     else if (type == 1) backward_shape<__bf16>(rows, F, tsh, nv, block, grid);
     else backward_shape<_Float16>(rows, F, tsh, nv, block, grid);
 }
+template <class T, bool EVEN, bool NT> void launch_backward_nv(const iso::RmsBackArgs& a, int nv, int block, int grid, hipStream_t s) {
+    if (nv == 1) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 1, EVEN, NT>), dim3(grid), dim3(block), 0, s, a);
+    else if (nv == 2) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 2, EVEN, NT>), dim3(grid), dim3(block), 0, s, a);
+    else hipLaunchKernelGGL((iso::rms_backward_kernel<T, 4, EVEN, NT>), dim3(grid), dim3(block), 0, s, a);
+}
 template <class T> void launch_backward(iso::RmsBackArgs a, int nv, int block, int grid, hipStream_t s) {
-    if (nv == 1) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 1>), dim3(grid), dim3(block), 0, s, a);
-    else if (nv == 2) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 2>), dim3(grid), dim3(block), 0, s, a);
-    else if (nv == 4) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 4>), dim3(grid), dim3(block), 0, s, a);
-    else {
-        if (a.ds)
-            for (a.row0 = 0; a.row0 < a.rows; a.row0 += MAX_THREADS / 512)
-                hipLaunchKernelGGL((iso::rms_backward_long_kernel<T>), dim3((unsigned)std::min(MAX_THREADS / 512, a.rows - a.row0)), dim3(512), 0, s, a);
-        if (a.dw_part) hipLaunchKernelGGL((iso::rms_dw_columns_kernel<T>), dim3((a.F + 255) / 256, grid), dim3(256), 0, s, a, grid);
+    if (nv != 0) {
+        const bool even = a.F % iso::RowVec<T>::N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= ROWS_NT_BYTES;
+        if (even && nt) launch_backward_nv<T, true, true>(a, nv, block, grid, s);
+        else if (even) launch_backward_nv<T, true, false>(a, nv, block, grid, s);
+        else if (nt) launch_backward_nv<T, false, true>(a, nv, block, grid, s);
+        else launch_backward_nv<T, false, false>(a, nv, block, grid, s);
+        return;
     }
+    if (a.ds)
+        for (a.row0 = 0; a.row0 < a.rows; a.row0 += MAX_THREADS / 512)
+            hipLaunchKernelGGL((iso::rms_backward_long_kernel<T>), dim3((unsigned)std::min(MAX_THREADS / 512, a.rows - a.row0)), dim3(512), 0, s, a);
+    if (a.dw_part) hipLaunchKernelGGL((iso::rms_dw_columns_kernel<T>), dim3((a.F + 255) / 256, grid), dim3(256), 0, s, a, grid);
 }
 template <class T, int CODE> void launch_read(iso::ReadArgs a, hipStream_t s) {
+    constexpr int N = iso::RowVec<T>::N;
     int nv;
-    row_shape((a.F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, a.rows, 2, 8, a.tsh, nv);
+    row_shape((a.F + N - 1) / N, a.rows, ROWS_LEAST_READ, 8, a.tsh, nv);
     a.tpr = 1 << a.tsh;
-    const int block = std::max(256, a.tpr);
-    const long long step = MAX_THREADS / block * (block / a.tpr);
+    const bool even = a.F % N == 0;
+    const int block = row_block(a.tsh), rpb = block >> a.tsh;
+    const long long step = MAX_THREADS / block * rpb;
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
-        const dim3 grid((unsigned)((n + block / a.tpr - 1) / (block / a.tpr)));
-#define READ(NV) hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV>), grid, dim3(block), 0, s, a)
-#define READ_LONG hipLaunchKernelGGL((iso::rows_read_long_kernel<T, CODE>), dim3((unsigned)n), dim3(512), 0, s, a)
-        ROWS_NV(nv, READ, READ_LONG);
+        const dim3 grid((unsigned)((n + rpb - 1) / rpb));
+#define READ(NV, EVEN) hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, EVEN>), grid, dim3(block), 0, s, a)
+#define READ_LONG hipLaunchKernelGGL((iso::rows_read_long_kernel<T, CODE>), grid, dim3(block), 0, s, a)
+        ROWS_NV(nv, even, READ, READ_LONG);
 #undef READ
 #undef READ_LONG
     }
