@@ -51,15 +51,15 @@ template <class T, int N> __device__ __forceinline__ void raw_float(const typena
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = (float)q[i];
 }
-template <class T, int N, bool EVEN> __device__ __forceinline__ void row_load(const T* row, int at, int F, bool on, float (&v)[N]) {
-    raw_float<T, N>(raw_load<T, N, EVEN>(row, at, F, on), v);
+template <class T, int N, bool EVEN, bool NT = false> __device__ __forceinline__ void row_load(const T* row, int at, int F, bool on, float (&v)[N]) {
+    raw_float<T, N>(raw_load<T, N, EVEN, NT>(row, at, F, on), v);
 }
 // v = x + res (res may be NULL)
-template <class T, int N, bool EVEN> __device__ __forceinline__ void sum_load(const T* x, const T* res, int at, int F, bool on, float (&v)[N]) {
-    row_load<T, N, EVEN>(x, at, F, on, v);
+template <class T, int N, bool EVEN, bool NT = false> __device__ __forceinline__ void sum_load(const T* x, const T* res, int at, int F, bool on, float (&v)[N]) {
+    row_load<T, N, EVEN, NT>(x, at, F, on, v);
     if (res) {
         float r[N];
-        row_load<T, N, EVEN>(res, at, F, on, r);
+        row_load<T, N, EVEN, NT>(res, at, F, on, r);
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] += r[i];
     }
@@ -263,14 +263,13 @@ template <int CODE> __device__ __forceinline__ unsigned encode4(const float* t, 
     }
     return in;
 }
-template <int N, bool EVEN> __device__ __forceinline__ void code_store(unsigned char* row, int at, int F, const unsigned (&c)[N / 4], int nt) {
+template <int N, bool EVEN> __device__ __forceinline__ void code_store(unsigned char* row, int at, int F, const unsigned (&c)[N / 4]) {
     typedef unsigned V __attribute__((ext_vector_type(N / 4), aligned(1)));
     if (EVEN || at + N <= F) {
         V q;
 #pragma unroll
         for (int i = 0; i < N / 4; i++) q[i] = c[i];
-        if (nt) __builtin_nontemporal_store(q, reinterpret_cast<V*>(row + at));
-        else *reinterpret_cast<V*>(row + at) = q;
+        *reinterpret_cast<V*>(row + at) = q;
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++)
@@ -328,7 +327,6 @@ struct RmsArgs {
     long long rows, row0;   // this launch starts at row row0
     int F, tpr, tsh, norm, w32;     // tpr = 1 << tsh threads per row
     int groups, gshift;     // groups per row and log2 of their columns; one group: 1 and 31
-    int nt;                 // codes past the caches
     float eps;
     double inv_F;
     const void* x;
@@ -343,7 +341,8 @@ struct RmsArgs {
     float* scales;          // [P, groups]
     RowTarget to;
 };
-template <class T, int NV, int OUT, bool EVEN> __global__ __launch_bounds__(512) void rms_forward_kernel(RmsArgs a) {
+// NT: the rows are read past the caches.
+template <class T, int NV, int OUT, bool EVEN, bool NT> __global__ __launch_bounds__(512) void rms_forward_kernel(RmsArgs a) {
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1);
@@ -353,7 +352,7 @@ template <class T, int NV, int OUT, bool EVEN> __global__ __launch_bounds__(512)
     const T* res = a.res ? (const T*)a.res + (on ? i : 0) * a.ldr : nullptr;
     float v[NV][N];
 #pragma unroll
-    for (int k = 0; k < NV; k++) sum_load<T, N, EVEN>(x, res, (t + k * tpr) * N, a.F, on, v[k]);
+    for (int k = 0; k < NV; k++) sum_load<T, N, EVEN, NT>(x, res, (t + k * tpr) * N, a.F, on, v[k]);
     float rstd = 1.0f;
     if (a.norm) {
         double wide;
@@ -390,7 +389,7 @@ template <class T, int NV, int OUT, bool EVEN> __global__ __launch_bounds__(512)
             unsigned c[N / 4];
 #pragma unroll
             for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[k][4 * q], g);
-            code_store<N, EVEN>(a.codes + row * a.F, at, a.F, c, a.nt);
+            code_store<N, EVEN>(a.codes + row * a.F, at, a.F, c);
             if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
         }
     }
@@ -445,7 +444,7 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
                 unsigned c[N / 4];
 #pragma unroll
                 for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[4 * q], g);
-                code_store<N, false>(a.codes + row * a.F, at, a.F, c, a.nt);
+                code_store<N, false>(a.codes + row * a.F, at, a.F, c);
                 if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
             }
         }
@@ -682,7 +681,8 @@ __device__ __forceinline__ long long read_row(const ReadArgs& a, long long i) {
     const long long row = a.index == nullptr ? a.first + i : a.is64 ? ((const long long*)a.index)[i] : (long long)((const int*)a.index)[i];
     return row < a.P ? row : -1;
 }
-template <class T, int CODE, int NV, bool EVEN> __global__ __launch_bounds__(512) void rows_read_kernel(ReadArgs a) {
+// NT: written past the caches.
+template <class T, int CODE, int NV, bool EVEN, bool NT> __global__ __launch_bounds__(512) void rows_read_kernel(ReadArgs a) {
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1);
@@ -703,7 +703,7 @@ template <class T, int CODE, int NV, bool EVEN> __global__ __launch_bounds__(512
         const int at = (t + k * tpr) * N;
 #pragma unroll
         for (int e = 0; e < N; e++) v[k][e] *= inv;
-        if (at < a.F) row_store<T, N, EVEN>((T*)a.out + i * a.F, at, a.F, v[k]);
+        if (at < a.F) row_store<T, N, EVEN, NT>((T*)a.out + i * a.F, at, a.F, v[k]);
     }
 }
 template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_long_kernel(ReadArgs a) {

@@ -19,24 +19,17 @@ bool code_type(int c) { return c == iso::CODE_INT8 || c == iso::CODE_E4M3; }
 bool group_ok(int F, int group) { return group == F || ((group == 32 || group == 64 || group == 128) && F % group == 0); }
 int group_shift(int F, int group) { return group == F ? 31 : group == 32 ? 5 : group == 64 ? 6 : 7; }
 
-#ifndef ROWS_GRID
-#define ROWS_GRID 512
-#endif
-#ifndef ROWS_LEAST_FWD
-#define ROWS_LEAST_FWD 1
-#endif
-#ifndef ROWS_LEAST_Q
-#define ROWS_LEAST_Q 2
-#endif
-#ifndef ROWS_LEAST_READ
-#define ROWS_LEAST_READ 2
-#endif
-#ifndef ROWS_NT_BYTES
-#define ROWS_NT_BYTES (128ll << 20)
-#endif
+// From this many bytes a stream is read (backward pass, 8-bit writes) or written (backward pass, 8-bit reads) past the caches: half of the
+// 256 MB last-level cache, so that it would push out more than the next kernel finds of it.  Measured on 1.28 GB / 134 MB streams: the whole
+// 8-bit table written and read 550 -> 530 us, rms_norm_quantized of [16384, 4096] bfloat16 94 -> 86, the backward pass of [8192, 8192] bfloat16
+// 149 -> 106, of [1.5 M, 32] float32 165 -> 132; a forward pass, whose outputs the next kernel reads, loses (128 -> 134) and keeps its lines.
+constexpr long long NT_BYTES = 128ll << 20;
+
 // threads per row (1 << tsh) and vectors per thread for a row of `vecs` vectors; 0 vectors per thread: the *_long form.
-// Within a wave `least` vectors per thread where there are rows enough to fill the chip all the same (what is done once per row weighs less);
-// beyond a wave 2 per thread; where there are so few rows that the chip would stand idle, up to 512 threads.
+// Within a wave `least` vectors per thread where there are rows enough to fill the chip all the same: 2 for 8-bit rows, whose work per row
+// (scales, the norm) weighs less then ([5 M, 64]: written 283 -> 258 us, read 359 -> 252; 4 are slower again, 64-byte pieces), 1 for the norm
+// ([1.5 M, 32]: 128 us, 160 with 2).  Beyond a wave 2 per thread ([8192, 8192] bfloat16: 240 us forward and backward, 333 with 4, 456 with 8).
+// Where there are so few rows that the chip would stand idle, up to 512 threads.
 void row_shape(int vecs, long long rows, int least, int max_nv, int& tsh, int& nv) {
     tsh = 0;
     while ((1 << tsh) < vecs && tsh < 6) tsh++;
@@ -57,16 +50,16 @@ int row_block(int tsh) { return tsh > 6 ? 1 << tsh : 256; }         // beyond a 
 template <class T, int OUT> void launch_forward(iso::RmsArgs a, hipStream_t s) {
     constexpr int N = iso::RowVec<T>::N;
     int nv;
-    row_shape((a.F + N - 1) / N, a.rows, OUT == 0 ? ROWS_LEAST_FWD : ROWS_LEAST_Q, 8, a.tsh, nv);
+    row_shape((a.F + N - 1) / N, a.rows, OUT == 0 ? 1 : 2, 8, a.tsh, nv);
     a.tpr = 1 << a.tsh;
-    a.nt = a.rows * a.F * (long long)sizeof(T) >= ROWS_NT_BYTES;
-    const bool even = a.F % N == 0;
+    const bool nt = OUT != 0 && a.rows * a.F * (long long)sizeof(T) >= NT_BYTES, even = a.F % N == 0;
     const int block = row_block(a.tsh), rpb = block >> a.tsh;
     const long long step = MAX_THREADS / block * rpb;
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
         const dim3 grid((unsigned)((n + rpb - 1) / rpb));
-#define FWD(NV, EVEN) hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, EVEN>), grid, dim3(block), 0, s, a)
+#define FWD(NV, EVEN) do { if (OUT != 0 && nt) hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, EVEN, OUT != 0>), grid, dim3(block), 0, s, a); \
+                           else hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, EVEN, false>), grid, dim3(block), 0, s, a); } while (0)
 #define FWD_LONG hipLaunchKernelGGL((iso::rms_forward_long_kernel<T, OUT>), grid, dim3(block), 0, s, a)
         ROWS_NV(nv, even, FWD, FWD_LONG);
 #undef FWD
@@ -90,7 +83,7 @@ template <class T> void backward_shape(long long rows, int F, int& tsh, int& nv,
     if (nv == 0) { grid = (int)std::min<long long>(64, std::max<long long>(1, rows)); return; }       // slices of the columns' sums
     const int rpb = block >> tsh;
     const long long need = (rows + rpb - 1) / rpb;
-    const long long most = std::max<long long>(ROWS_GRID, std::min<long long>(2048, (1 << 20) / F));
+    const long long most = std::max<long long>(512, std::min<long long>(2048, (1 << 20) / F));
     grid = (int)std::max<long long>(1, std::min(need, most));
 }
 void backward_shape_type(int type, long long rows, int F, int& tsh, int& nv, int& block, int& grid) {
@@ -105,7 +98,7 @@ template <class T, bool EVEN, bool NT> void launch_backward_nv(const iso::RmsBac
 }
 template <class T> void launch_backward(iso::RmsBackArgs a, int nv, int block, int grid, hipStream_t s) {
     if (nv != 0) {
-        const bool even = a.F % iso::RowVec<T>::N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= ROWS_NT_BYTES;
+        const bool even = a.F % iso::RowVec<T>::N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= NT_BYTES;
         if (even && nt) launch_backward_nv<T, true, true>(a, nv, block, grid, s);
         else if (even) launch_backward_nv<T, true, false>(a, nv, block, grid, s);
         else if (nt) launch_backward_nv<T, false, true>(a, nv, block, grid, s);
@@ -120,15 +113,16 @@ template <class T> void launch_backward(iso::RmsBackArgs a, int nv, int block, i
 template <class T, int CODE> void launch_read(iso::ReadArgs a, hipStream_t s) {
     constexpr int N = iso::RowVec<T>::N;
     int nv;
-    row_shape((a.F + N - 1) / N, a.rows, ROWS_LEAST_READ, 8, a.tsh, nv);
+    row_shape((a.F + N - 1) / N, a.rows, 2, 8, a.tsh, nv);
     a.tpr = 1 << a.tsh;
-    const bool even = a.F % N == 0;
+    const bool even = a.F % N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= NT_BYTES;
     const int block = row_block(a.tsh), rpb = block >> a.tsh;
     const long long step = MAX_THREADS / block * rpb;
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
         const dim3 grid((unsigned)((n + rpb - 1) / rpb));
-#define READ(NV, EVEN) hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, EVEN>), grid, dim3(block), 0, s, a)
+#define READ(NV, EVEN) do { if (nt) hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, EVEN, true>), grid, dim3(block), 0, s, a); \
+                            else hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, EVEN, false>), grid, dim3(block), 0, s, a); } while (0)
 #define READ_LONG hipLaunchKernelGGL((iso::rows_read_long_kernel<T, CODE>), grid, dim3(block), 0, s, a)
         ROWS_NV(nv, even, READ, READ_LONG);
 #undef READ

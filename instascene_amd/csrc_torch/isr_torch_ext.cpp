@@ -170,8 +170,12 @@ torch::Tensor markVisible(torch::Tensor& means3D_, torch::Tensor& viewmatrix_, t
     return present;
 }
 
+void bind_rows(pybind11::module_& m);       // isr_torch_rows.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    m.doc() = "diff_surfel_rasterization._C for MI355X: the reference's three entry points on libinstascene_hip.so";
+    m.doc() = "diff_surfel_rasterization._C for MI355X: the reference's three entry points on libinstascene_hip.so, and the host side of "
+              "instascene_amd.rows / the gradient norm of instascene_amd.optim";
+    bind_rows(m);
     m.def("rasterize_gaussians", &RasterizeGaussiansHIP);
     m.def("rasterize_gaussians_backward", &RasterizeGaussiansBackwardHIP);
     m.def("mark_visible", &markVisible);

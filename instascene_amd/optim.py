@@ -19,13 +19,13 @@ Beside it, for any list of gradients: their global norm (:func:`grad_norm`) and 
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import Dict, Iterable, Optional, Sequence
 
 import torch
 
 from . import _hot
 from ._lib import check, lib
+from .rows import _ext
 
 GROUPS = ("xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation")
 _ATTR = {"xyz": "_xyz", "f_dc": "_features_dc", "f_rest": "_features_rest", "opacity": "_opacity", "scaling": "_scaling",
@@ -138,66 +138,13 @@ class GaussianAdam:
 
 
 # -- the global norm of many gradients, and clipping ----------------------------------------------------------------------------
-_GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_NORM_TYPES = {1.0: 1, 2.0: 2, math.inf: 0}
-
-
-def _is_dense(t: torch.Tensor) -> bool:
-    """Whether the elements fill one stretch of memory, each once (in any order of the dimensions)."""
-    if t.is_contiguous():
-        return True
-    expect = 1
-    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
-        if stride != expect:
-            return False
-        expect *= size
-    return True
-
-
-def _norm_launch(what, tensors, norm_type, max_norm, clip):
-    kind = _NORM_TYPES.get(float(norm_type))
-    if kind is None:
-        raise ValueError(f"{what}: norm_type must be 1, 2 or inf, not {norm_type}")
-    dev = tensors[0].device
-    flat, back = [], []
-    for t in tensors:
-        if t.layout != torch.strided or not t.is_cuda:
-            raise RuntimeError(f"{what}: needs dense CUDA tensors (the HIP library is the only backend)")
-        if t.dtype not in _GRAD_TYPES:
-            raise TypeError(f"{what}: float32, bfloat16 or float16 gradients, not {t.dtype}")
-        if t.device != dev:
-            raise ValueError(f"{what}: all gradients must be on one device, not {dev} and {t.device}")
-        if not _is_dense(t):
-            if clip and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-                raise ValueError(f"{what}: an expanded tensor cannot be clipped in place")
-            c = t.contiguous()
-            back.append((t, c))
-            t = c
-        flat.append(t)
-    n = len(flat)
-    sizes = (ctypes.c_longlong * n)(*[t.numel() for t in flat])
-    L = lib()
-    nbytes = L.iso_grad_norm_scratch_bytes(n, sizes)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    out = torch.empty(2, dtype=torch.float32, device=dev)
-    with _hot.on_device(dev):
-        check(L.iso_grad_norm(n, (ctypes.c_void_p * n)(*[t.data_ptr() for t in flat]), sizes,
-                              (ctypes.c_int * n)(*[_GRAD_TYPES[t.dtype] for t in flat]), kind, float(max_norm), int(clip), out.data_ptr(),
-                              scratch.data_ptr(), nbytes, _hot.raw_stream(dev)), "iso_grad_norm")
-    if clip:
-        torch.autograd.graph.increment_version(flat)         # the kernel wrote through raw pointers
-        for t, c in back:
-            t.copy_(c)
-    return out
-
-
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """The norm (2, 1 or inf) of all elements of ``tensors`` together, as a float32 scalar on their device; nothing is synchronised.
     float32, bfloat16 and float16 may be mixed; sums are held in 64 bits.  No tensors: 0."""
-    tensors = [t.detach() for t in ([tensors] if isinstance(tensors, torch.Tensor) else tensors)]
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         return torch.tensor(0.0)
-    return _norm_launch("grad_norm", tensors, norm_type, 0.0, False)[0]
+    return _ext().grad_norm(tensors, norm_type, 0.0, False)
 
 
 def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
@@ -205,7 +152,7 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
     ``torch.nn.utils.clip_grad_norm_`` does, on a list of gradients.  The factor stays on the device; gradients that need no clipping are
     read once and not written.  Two of them may not share memory.  ``error_if_nonfinite`` reads the norm back (a synchronisation) and
     raises before anything is scaled."""
-    grads = [g.detach() for g in ([grads] if isinstance(grads, torch.Tensor) else grads)]
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads_: max_norm must not be negative, is {max_norm}")
@@ -215,7 +162,7 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
         norm = grad_norm(grads, norm_type)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"clip_grads_: the norm of order {norm_type} of the gradients is {float(norm)}; nothing was clipped")
-    return _norm_launch("clip_grads_", grads, norm_type, max_norm, True)[0]
+    return _ext().grad_norm(grads, norm_type, max_norm, True)
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
