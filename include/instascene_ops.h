@@ -258,6 +258,21 @@ size_t iso_grad_norm_scratch_bytes(int count, const long long* sizes);
 int iso_grad_norm(int count, void* const* tensors, const long long* sizes, const int* types, int norm_type, float max_norm, int clip,
                   float* out /*[2]*/, void* scratch, size_t scratch_bytes, void* stream);
 
+/* The same norm (type 2) for the six parameter groups of iso_gaussian_adam_step, of the RAW parameters' gradients: its chain rule applied to the
+ * gradients of the activated tensors on the way.  out[0] = norm, out[1] = coef.  scratch: iso_grad_norm_scratch_bytes(1, NULL). */
+int iso_gaussian_grad_norm(int P, int M, float* const params[6], const float* g_xyz, const float* g_shs, const float* g_opacity,
+                           const float* g_scale, const float* g_rotation, float max_norm, float* out /*[2]*/, void* scratch, size_t scratch_bytes,
+                           void* stream);
+/* iso_adam_rownorm2 / iso_gaussian_adam_step with every parameter's gradient times *coef (a device float: out + 1 of the norms above) on the
+ * way: clipping without a pass of its own.  coef NULL: the plain step. */
+int iso_adam_rownorm2_clipped(long long N, int F, double lr, double beta1, double beta2, double eps, long long step, float eps1,
+                              float eps2, float* param, const float* grad, float* exp_avg, float* exp_avg_sq, float* y, float* z,
+                              const float* coef, void* stream);
+int iso_gaussian_adam_step_clipped(int P, int M, float* const params[6], float* const exp_avg[6], float* const exp_avg_sq[6],
+                                   const double lr[6], double beta1, double beta2, double eps, long long step, const float* g_xyz,
+                                   const float* g_shs, const float* g_opacity, const float* g_scale, const float* g_rotation,
+                                   float* a_shs, float* a_opacity, float* a_scale, float* a_rotation, const float* coef, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -123,6 +123,11 @@ SIGNATURES = {
                                c_float, _P, _P]),
     "iso_grad_norm_scratch_bytes": (c_size_t, [c_int, _P]),
     "iso_grad_norm": (c_int, [c_int, _P, _P, _P, c_int, c_float, c_int, _P, _P, c_size_t, _P]),
+    "iso_gaussian_grad_norm": (c_int, [c_int, c_int, _P, _P, _P, _P, _P, _P, c_float, _P, _P, c_size_t, _P]),
+    "iso_adam_rownorm2_clipped": (c_int, [ctypes.c_longlong, c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                                          ctypes.c_longlong, c_float, c_float, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "iso_gaussian_adam_step_clipped": (c_int, [c_int, c_int, _P, _P, _P, _P, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                                               ctypes.c_longlong, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "iso_rownorm2": (c_int, [ctypes.c_longlong, c_int, c_float, c_float, c_int, _P, _P, _P, _P, _P, _P]),
 }
 

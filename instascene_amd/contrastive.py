@@ -363,6 +363,7 @@ class FeatureAdam:
         self.exp_avg = torch.zeros_like(param, memory_format=torch.contiguous_format)
         self.exp_avg_sq = torch.zeros_like(param, memory_format=torch.contiguous_format)
         self.step_count = 0
+        self.last_grad_norm = None      # of the last step with max_grad_norm: a float32 scalar on the device
         self.normalized = None          # (version of param, y, z) written by the last step
         # leaf mode (``step_rows``): normalized_chain() hands out y and z as LEAVES; the caller finishes the chain rule,
         # the optimiser step and the next normalisation in one pass over the rows (isr_feature_rows_step)
@@ -383,36 +384,58 @@ class FeatureAdam:
         self._zscale = None
         self._zplace = None
 
-    def step(self):
+    def _clip_coef(self, grads, max_grad_norm):
+        from .optim import check_max_norm, norm_and_coef
+        self.last_grad_norm, coef = norm_and_coef(grads, check_max_norm("FeatureAdam", max_grad_norm))
+        return coef
+
+    def step(self, max_grad_norm=None):
+        """``max_grad_norm``: the gradient clipped to this 2-norm on its way into the step (``p.grad`` itself stays as it is); the norm is
+        then in ``last_grad_norm``."""
         p = self.param
         if p.grad is None:
             return
+        coef = None if max_grad_norm is None else self._clip_coef([p.grad], max_grad_norm)
         L = lib()
         g = p.grad.contiguous().float()
         y, z = torch.empty_like(p.data), torch.empty_like(p.data)
         self.step_count += 1
         with _hot.on_device(p.device):
-            check(L.iso_adam_rownorm2(p.shape[0], p.shape[1], self.lr, float(self.betas[0]), float(self.betas[1]), self.eps,
-                                      self.step_count, float(self.norm_eps[0]), float(self.norm_eps[1]), _p(p.data), _p(g),
-                                      _p(self.exp_avg), _p(self.exp_avg_sq), _p(y), _p(z), _stream()), "iso_adam_rownorm2")
+            check(L.iso_adam_rownorm2_clipped(p.shape[0], p.shape[1], self.lr, float(self.betas[0]), float(self.betas[1]), self.eps,
+                                              self.step_count, float(self.norm_eps[0]), float(self.norm_eps[1]), _p(p.data), _p(g),
+                                              _p(self.exp_avg), _p(self.exp_avg_sq), _p(y), _p(z), _p(coef), _stream()),
+                  "iso_adam_rownorm2")
         torch.autograd.graph.increment_version(p)       # the kernel wrote through the raw pointer: tell autograd
         self.normalized = (p._version, y, z)
 
-    def step_rows(self, rows=None, grad_only: bool = False, row_grads=None, dense=None):
+    def step_rows(self, rows=None, grad_only: bool = False, row_grads=None, dense=None, max_grad_norm=None):
         """Leaf mode: finish the step from the gradients that reached the leaves of ``normalized_chain()`` — ``y.grad``
         (3-D loss), ``z.grad`` (any dense rasterizer gradient) — and the partial rows ``rows`` a
         ``rasterizer.DeferredFeatureRows`` block collected: reduction, chain rule through both normalisations, Adam and
         the next normalisations in ONE kernel (``isr_feature_rows_step``).  ``grad_only``: stop at ``param.grad`` (for an
         all-reduce; ``step()`` then completes).  ``row_grads``: sparse gradient on ``y`` rows — ``(idx int64, [n,F])``, or
-        the ``(slot int32 [P], merged [n,F])`` pair ``compact_row_grads`` makes of it (``gather_rows`` does so itself)."""
+        the ``(slot int32 [P], merged [n,F])`` pair ``compact_row_grads`` makes of it (``gather_rows`` does so itself).
+        ``max_grad_norm``: clip the gradient to this 2-norm; the norm has to be known before the first row is stepped, so the gradient is
+        materialised and the step is a pass of its own (``clipped_step``)."""
         tail = self.begin_tail(rows, row_grads, dense)
         if tail is None:
             return
         P = self.param.shape[0]
         if grad_only:
             self.tail_gradient(tail, 0, P)
+        elif max_grad_norm is not None:
+            self.tail_gradient(tail, 0, P)
+            self.clipped_step(max_grad_norm)
+            self.param.grad = None
         else:
             self.tail_update(tail)
+
+    def clipped_step(self, max_grad_norm):
+        """The step from ``param.grad`` clipped to ``max_grad_norm``, with the outputs a leaf-mode step leaves behind."""
+        coef = self._clip_coef([self.param.grad], max_grad_norm)
+        self.begin_step()
+        self.step_range(0, self.param.shape[0], coef=coef)
+        self.end_step()
 
     # -- the tail in pieces (a data-parallel trainer walks the table in row ranges: see SegTrainer) ------------------
     def begin_tail(self, rows=None, row_grads=None, dense=None):
@@ -494,9 +517,10 @@ class FeatureAdam:
         self.step_count += 1
         self._pending_yz = (torch.empty_like(p.data) if self.store_y else None, torch.empty_like(p.data))
 
-    def step_range(self, r0: int, r1: int, grad_rows=None):
+    def step_range(self, r0: int, r1: int, grad_rows=None, coef=None):
         """Adam + the two normalisations on rows ``[r0, r1)`` from ``param.grad`` (``iso_adam_rownorm2`` on the slice), or
-        from ``grad_rows [r1 - r0, F]`` when the summed gradient of those rows lives elsewhere (a reduce-scatter's shard)."""
+        from ``grad_rows [r1 - r0, F]`` when the summed gradient of those rows lives elsewhere (a reduce-scatter's shard).
+        ``coef``: a device float that every gradient is multiplied by (clipping)."""
         p = self.param
         if r1 <= r0:
             return
@@ -505,9 +529,9 @@ class FeatureAdam:
         at = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr() + 4 * F * int(r0))
         g = at(p.grad) if grad_rows is None else _p(grad_rows.contiguous())
         with _hot.on_device(p.device):
-            check(lib().iso_adam_rownorm2(int(r1 - r0), F, self.lr, float(self.betas[0]), float(self.betas[1]), self.eps,
-                                          self.step_count, float(self.norm_eps[0]), float(self.norm_eps[1]), at(p.data),
-                                          g, at(self.exp_avg), at(self.exp_avg_sq), at(y), at(z), _stream()),
+            check(lib().iso_adam_rownorm2_clipped(int(r1 - r0), F, self.lr, float(self.betas[0]), float(self.betas[1]), self.eps,
+                                                  self.step_count, float(self.norm_eps[0]), float(self.norm_eps[1]), at(p.data),
+                                                  g, at(self.exp_avg), at(self.exp_avg_sq), at(y), at(z), _p(coef), _stream()),
                   "iso_adam_rownorm2")
 
     def renormalize_range(self, r0: int, r1: int):

@@ -689,11 +689,13 @@ __device__ __forceinline__ void iso_nt_store4(float* p, const float4& v) {
     const iso_nt_f4 q = {v.x, v.y, v.z, v.w};
     __builtin_nontemporal_store(q, reinterpret_cast<iso_nt_f4*>(p));
 }
+// CLIP: every gradient times *coef first (what iso_grad_norm left for it), so that clipping costs no pass of its own.
+template <bool CLIP>
 __global__ __launch_bounds__(256) void adam_rn2_kernel(long long N, int F, float lr_over_bc1, float om1, float beta2, float om2,
                                                        float inv_sqrt_bc2, float eps, float eps1, float eps2,
                                                        float* __restrict__ p, const float* __restrict__ g,
                                                        float* __restrict__ m, float* __restrict__ v,
-                                                       float* __restrict__ y, float* __restrict__ z) {
+                                                       float* __restrict__ y, float* __restrict__ z, const float* __restrict__ coef) {
     const int q = F >> 2;
     int lpr = 1;
     while (lpr < q) lpr <<= 1;
@@ -703,7 +705,9 @@ __global__ __launch_bounds__(256) void adam_rn2_kernel(long long N, int F, float
     const size_t off = (size_t)(row < N ? row : 0) * F + 4 * sub;
     float4 np4 = make_float4(0, 0, 0, 0);
     if (ok) {
-        const float4 p4 = *reinterpret_cast<const float4*>(p + off), g4 = *reinterpret_cast<const float4*>(g + off);
+        const float4 p4 = *reinterpret_cast<const float4*>(p + off);
+        float4 g4 = *reinterpret_cast<const float4*>(g + off);
+        if (CLIP) { const float c = *coef; g4.x *= c; g4.y *= c; g4.z *= c; g4.w *= c; }
         float4 m4 = iso_nt_load4(m + off), v4 = iso_nt_load4(v + off);
 #define ISO_ADAM1(c)                                                                   \
         m4.c = m4.c + om1 * (g4.c - m4.c);                                             \

@@ -33,11 +33,14 @@ struct GaussAdamArgs {
     float* a_opa;
     float* a_scale;
     float* a_rot;
+    const float* coef;     // CLIP: the raw parameters' gradients times *coef
     float om1, beta2, om2, inv_sqrt_bc2, eps;
     int P, M;      // M = SH coefficients per colour (16 for degree 3); R = 3 (M - 1)
 };
 
+template <bool CLIP>
 __device__ __forceinline__ float adam1(float& p, float g, float& m, float& v, float lr_over_bc1, const GaussAdamArgs& a) {
+    if (CLIP) g *= *a.coef;
     m = m + a.om1 * (g - m);
     v = a.beta2 * v + a.om2 * (g * g);
     p = p - lr_over_bc1 * (m / (__builtin_sqrtf(v) * a.inv_sqrt_bc2 + a.eps));
@@ -45,13 +48,14 @@ __device__ __forceinline__ float adam1(float& p, float g, float& m, float& v, fl
 }
 
 // thread space: [0, 3P) xyz | [3P, 3P + 3MP) sh coefficients | P opacity | 2P scaling | P rotation rows
+template <bool CLIP>
 __global__ __launch_bounds__(256) void gaussian_adam_kernel(GaussAdamArgs a) {
     const long long P = a.P, S = 3LL * a.M;
     long long e = (long long)blockIdx.x * 256 + threadIdx.x;
     if (e < 3 * P) {                                        // xyz: identity activation
         if (a.g_xyz == nullptr) return;
         float p = a.p[0][e], m = a.m[0][e], v = a.v[0][e];
-        adam1(p, a.g_xyz[e], m, v, a.lr_over_bc1[0], a);
+        adam1<CLIP>(p, a.g_xyz[e], m, v, a.lr_over_bc1[0], a);
         a.p[0][e] = p; a.m[0][e] = m; a.v[0][e] = v;
         return;
     }
@@ -64,7 +68,7 @@ __global__ __launch_bounds__(256) void gaussian_adam_kernel(GaussAdamArgs a) {
         float p = a.p[grp][off];
         if (a.g_shs != nullptr) {
             float m = a.m[grp][off], v = a.v[grp][off];
-            adam1(p, a.g_shs[e], m, v, a.lr_over_bc1[grp], a);
+            adam1<CLIP>(p, a.g_shs[e], m, v, a.lr_over_bc1[grp], a);
             a.p[grp][off] = p; a.m[grp][off] = m; a.v[grp][off] = v;
         }
         if (a.a_shs != nullptr) a.a_shs[e] = p;
@@ -76,7 +80,7 @@ __global__ __launch_bounds__(256) void gaussian_adam_kernel(GaussAdamArgs a) {
         if (a.g_opa != nullptr) {
             const float s = 1.0f / (1.0f + expf(-p));
             float m = a.m[3][e], v = a.v[3][e];
-            adam1(p, a.g_opa[e] * (s * (1.0f - s)), m, v, a.lr_over_bc1[3], a);
+            adam1<CLIP>(p, a.g_opa[e] * (s * (1.0f - s)), m, v, a.lr_over_bc1[3], a);
             a.p[3][e] = p; a.m[3][e] = m; a.v[3][e] = v;
         }
         if (a.a_opa != nullptr) a.a_opa[e] = 1.0f / (1.0f + expf(-p));
@@ -87,7 +91,7 @@ __global__ __launch_bounds__(256) void gaussian_adam_kernel(GaussAdamArgs a) {
         float p = a.p[4][e];
         if (a.g_scale != nullptr) {
             float m = a.m[4][e], v = a.v[4][e];
-            adam1(p, a.g_scale[e] * expf(p), m, v, a.lr_over_bc1[4], a);
+            adam1<CLIP>(p, a.g_scale[e] * expf(p), m, v, a.lr_over_bc1[4], a);
             a.p[4][e] = p; a.m[4][e] = m; a.v[4][e] = v;
         }
         if (a.a_scale != nullptr) a.a_scale[e] = expf(p);
@@ -103,10 +107,10 @@ __global__ __launch_bounds__(256) void gaussian_adam_kernel(GaussAdamArgs a) {
             const float d = y.x * g.x + y.y * g.y + y.z * g.z + y.w * g.w;
             const float4 gq = make_float4((g.x - y.x * d) * r, (g.y - y.y * d) * r, (g.z - y.z * d) * r, (g.w - y.w * d) * r);
             float4 m = reinterpret_cast<const float4*>(a.m[5])[e], v = reinterpret_cast<const float4*>(a.v[5])[e];
-            adam1(q.x, gq.x, m.x, v.x, a.lr_over_bc1[5], a);
-            adam1(q.y, gq.y, m.y, v.y, a.lr_over_bc1[5], a);
-            adam1(q.z, gq.z, m.z, v.z, a.lr_over_bc1[5], a);
-            adam1(q.w, gq.w, m.w, v.w, a.lr_over_bc1[5], a);
+            adam1<CLIP>(q.x, gq.x, m.x, v.x, a.lr_over_bc1[5], a);
+            adam1<CLIP>(q.y, gq.y, m.y, v.y, a.lr_over_bc1[5], a);
+            adam1<CLIP>(q.z, gq.z, m.z, v.z, a.lr_over_bc1[5], a);
+            adam1<CLIP>(q.w, gq.w, m.w, v.w, a.lr_over_bc1[5], a);
             reinterpret_cast<float4*>(a.p[5])[e] = q;
             reinterpret_cast<float4*>(a.m[5])[e] = m;
             reinterpret_cast<float4*>(a.v[5])[e] = v;

@@ -347,9 +347,9 @@ int iso_densify_stats(int P, int C, const float* viewspace_grad, const unsigned 
     return ISR_OK;
 }
 
-int iso_adam_rownorm2(long long N, int F, double lr, double beta1, double beta2, double eps, long long step, float eps1,
-                      float eps2, float* param, const float* grad, float* exp_avg, float* exp_avg_sq, float* y, float* z,
-                      void* stream) {
+int iso_adam_rownorm2_clipped(long long N, int F, double lr, double beta1, double beta2, double eps, long long step, float eps1,
+                              float eps2, float* param, const float* grad, float* exp_avg, float* exp_avg_sq, float* y, float* z,
+                              const float* coef, void* stream) {
     hipStream_t s = (hipStream_t)stream;
     if (N < 0 || F <= 0 || (F & 3) != 0 || F > 256) return fail(ISR_EINVAL, "adam_rownorm2 needs F % 4 == 0 and F <= 256");
     if (step < 1) return fail(ISR_EINVAL, "adam_rownorm2: step counts from 1");
@@ -360,17 +360,26 @@ int iso_adam_rownorm2(long long N, int F, double lr, double beta1, double beta2,
     while (lpr < q) lpr <<= 1;
     const unsigned blocks = (unsigned)((N * lpr + 255) / 256);
     // hyper-parameters are doubles like torch's: 1 - 0.999f would be off by 5e-5 relative
-    hipLaunchKernelGGL(iso::adam_rn2_kernel, dim3(blocks), dim3(256), 0, s, N, F, (float)(lr / bc1), (float)(1.0 - beta1),
-                       (float)beta2, (float)(1.0 - beta2), (float)(1.0 / sqrt(bc2)), (float)eps, eps1, eps2, param, grad,
-                       exp_avg, exp_avg_sq, y, z);
+    const float f_lr = (float)(lr / bc1), om1 = (float)(1.0 - beta1), om2 = (float)(1.0 - beta2), isb = (float)(1.0 / sqrt(bc2));
+    if (coef)
+        hipLaunchKernelGGL(iso::adam_rn2_kernel<true>, dim3(blocks), dim3(256), 0, s, N, F, f_lr, om1, (float)beta2, om2, isb, (float)eps, eps1, eps2,
+                           param, grad, exp_avg, exp_avg_sq, y, z, coef);
+    else
+        hipLaunchKernelGGL(iso::adam_rn2_kernel<false>, dim3(blocks), dim3(256), 0, s, N, F, f_lr, om1, (float)beta2, om2, isb, (float)eps, eps1, eps2,
+                           param, grad, exp_avg, exp_avg_sq, y, z, coef);
     ISR_LAUNCH_CHECK("iso_adam_rownorm2");
     return ISR_OK;
 }
+int iso_adam_rownorm2(long long N, int F, double lr, double beta1, double beta2, double eps, long long step, float eps1,
+                      float eps2, float* param, const float* grad, float* exp_avg, float* exp_avg_sq, float* y, float* z,
+                      void* stream) {
+    return iso_adam_rownorm2_clipped(N, F, lr, beta1, beta2, eps, step, eps1, eps2, param, grad, exp_avg, exp_avg_sq, y, z, nullptr, stream);
+}
 
-int iso_gaussian_adam_step(int P, int M, float* const params[6], float* const exp_avg[6], float* const exp_avg_sq[6],
-                           const double lr[6], double beta1, double beta2, double eps, long long step, const float* g_xyz,
-                           const float* g_shs, const float* g_opacity, const float* g_scale, const float* g_rotation,
-                           float* a_shs, float* a_opacity, float* a_scale, float* a_rotation, void* stream) {
+int iso_gaussian_adam_step_clipped(int P, int M, float* const params[6], float* const exp_avg[6], float* const exp_avg_sq[6],
+                                   const double lr[6], double beta1, double beta2, double eps, long long step, const float* g_xyz,
+                                   const float* g_shs, const float* g_opacity, const float* g_scale, const float* g_rotation,
+                                   float* a_shs, float* a_opacity, float* a_scale, float* a_rotation, const float* coef, void* stream) {
     if (P < 0 || M < 1 || M > 64) return fail(ISR_EINVAL, "gaussian_adam_step: bad sizes P=%d M=%d", P, M);
     if (step < 1) return fail(ISR_EINVAL, "gaussian_adam_step: step counts from 1");
     if (P == 0) return ISR_OK;
@@ -389,9 +398,19 @@ int iso_gaussian_adam_step(int P, int M, float* const params[6], float* const ex
     a.inv_sqrt_bc2 = (float)(1.0 / sqrt(bc2)); a.eps = (float)eps;
     a.P = P; a.M = M;
     const long long threads = (long long)P * (3 + 3LL * M + 1 + 2 + 1);
-    hipLaunchKernelGGL(iso::gaussian_adam_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
+    a.coef = coef;
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    if (coef) hipLaunchKernelGGL(iso::gaussian_adam_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(iso::gaussian_adam_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, a);
     ISR_LAUNCH_CHECK_S("iso_gaussian_adam_step", (hipStream_t)stream);
     return ISR_OK;
+}
+int iso_gaussian_adam_step(int P, int M, float* const params[6], float* const exp_avg[6], float* const exp_avg_sq[6],
+                           const double lr[6], double beta1, double beta2, double eps, long long step, const float* g_xyz,
+                           const float* g_shs, const float* g_opacity, const float* g_scale, const float* g_rotation,
+                           float* a_shs, float* a_opacity, float* a_scale, float* a_rotation, void* stream) {
+    return iso_gaussian_adam_step_clipped(P, M, params, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, step, g_xyz, g_shs, g_opacity, g_scale,
+                                          g_rotation, a_shs, a_opacity, a_scale, a_rotation, nullptr, stream);
 }
 
 int iso_gather_rownorm(int n, int F, long long P, float eps, const float* x, const long long* idx, float* out, void* stream) {

@@ -287,7 +287,13 @@ int iso_grad_norm(int count, void* const* tensors, const long long* sizes, const
         if (overlap) return fail(ISR_EINVAL, "grad_norm: two of the tensors to be clipped share memory");
     }
     double* part = (double*)scratch;
-    int parts = 0;
+    int parts = 0, filled = 0;
+    long long total = 0;
+    for (int i = 0; i < count; i++) {
+        filled += sizes[i] > 0;
+        total = std::min(total + sizes[i], 1ll << 40);
+    }
+    const bool small = filled <= 16 && total <= iso::GN_SMALL;       // one workgroup, one launch
     for (int pass = 0; pass < (clip ? 2 : 1); pass++) {
         bool launched = false;
         for (int i = 0; i < count;) {
@@ -296,7 +302,10 @@ int iso_grad_norm(int count, void* const* tensors, const long long* sizes, const
             tb.count = 0;
             for (; i < count && tb.count < iso::GN_TENSORS; i++) {
                 if (sizes[i] == 0) continue;
-                const unsigned long long c = ((unsigned long long)sizes[i] + iso::GN_CHUNK - 1) / iso::GN_CHUNK;
+                const int size = type_bytes(types[i]);
+                const long long head = std::min<long long>((16 - ((uintptr_t)tensors[i] & 15)) % 16 / size, sizes[i]);
+                const unsigned long long c = std::max<unsigned long long>(1, ((unsigned long long)(sizes[i] - head) + iso::GN_CHUNK - 1) / iso::GN_CHUNK);
+                tb.head[tb.count] = (unsigned char)head;
                 if (chunks + c > 0xffffffffull) return fail(ISR_EINVAL, "grad_norm: too many elements");
                 tb.p[tb.count] = tensors[i]; tb.n[tb.count] = sizes[i]; tb.type[tb.count] = (unsigned char)types[i];
                 tb.first[tb.count++] = (unsigned)chunks;
@@ -305,6 +314,13 @@ int iso_grad_norm(int count, void* const* tensors, const long long* sizes, const
             if (tb.count == 0) break;
             tb.first[tb.count] = (unsigned)chunks;
             launched = true;
+            if (small) {
+                if (norm_type == 2) hipLaunchKernelGGL(iso::grad_small_kernel<2>, dim3(1), dim3(1024), 0, s, tb, clip, max_norm, out);
+                else if (norm_type == 1) hipLaunchKernelGGL(iso::grad_small_kernel<1>, dim3(1), dim3(1024), 0, s, tb, clip, max_norm, out);
+                else hipLaunchKernelGGL(iso::grad_small_kernel<0>, dim3(1), dim3(1024), 0, s, tb, clip, max_norm, out);
+                ISR_LAUNCH_CHECK("iso_grad_norm");
+                return ISR_OK;
+            }
             if (pass == 0) {
                 const int grid = (int)std::min<unsigned long long>(chunks, iso::GN_PARTS);
                 if (norm_type == 2) hipLaunchKernelGGL(iso::grad_norm_kernel<2>, dim3(grid), dim3(iso::GN_THREADS), 0, s, tb, part + parts);
@@ -312,7 +328,7 @@ int iso_grad_norm(int count, void* const* tensors, const long long* sizes, const
                 else hipLaunchKernelGGL(iso::grad_norm_kernel<0>, dim3(grid), dim3(iso::GN_THREADS), 0, s, tb, part + parts);
                 parts += grid;
             } else {
-                const int grid = (int)std::min<unsigned long long>(chunks, 2048);
+                const int grid = (int)std::min<unsigned long long>(chunks, 1024);
                 if (norm_type == 2) hipLaunchKernelGGL(iso::grad_clip_kernel<2>, dim3(grid), dim3(iso::GN_THREADS), 0, s, tb, part, parts, max_norm, out);
                 else if (norm_type == 1) hipLaunchKernelGGL(iso::grad_clip_kernel<1>, dim3(grid), dim3(iso::GN_THREADS), 0, s, tb, part, parts, max_norm, out);
                 else hipLaunchKernelGGL(iso::grad_clip_kernel<0>, dim3(grid), dim3(iso::GN_THREADS), 0, s, tb, part, parts, max_norm, out);
@@ -327,6 +343,28 @@ int iso_grad_norm(int count, void* const* tensors, const long long* sizes, const
             break;
         }
     }
+    return ISR_OK;
+}
+
+int iso_gaussian_grad_norm(int P, int M, float* const params[6], const float* g_xyz, const float* g_shs, const float* g_opacity,
+                           const float* g_scale, const float* g_rotation, float max_norm, float* out, void* scratch, size_t scratch_bytes,
+                           void* stream) {
+    hipStream_t s = (hipStream_t)stream;
+    if (P < 0 || M < 1 || M > 64) return fail(ISR_EINVAL, "gaussian_grad_norm: bad sizes P=%d M=%d", P, M);
+    if (!params || !out || !(max_norm >= 0.0f)) return fail(ISR_EINVAL, "gaussian_grad_norm: null argument, or max_norm negative");
+    if (!scratch || scratch_bytes < iso_grad_norm_scratch_bytes(1, nullptr)) return fail(ISR_EINVAL, "gaussian_grad_norm: scratch too small");
+    if (P > 0 && ((g_opacity && !params[3]) || (g_scale && !params[4]) || (g_rotation && !params[5]))) return fail(ISR_EINVAL, "gaussian_grad_norm: a gradient without its parameter");
+    if (((uintptr_t)g_rotation | (g_rotation ? (uintptr_t)params[5] : 0)) & 15) return fail(ISR_EINVAL, "gaussian_grad_norm: rotations must be 16-byte aligned");
+    double* part = (double*)scratch;
+    int parts = 0;
+    if (P > 0) {
+        iso::GaussNormArgs a = {P, 3ll * M * P, g_xyz, g_shs, g_opacity, g_scale, g_rotation, params[3], params[4], params[5]};
+        parts = (int)std::min<long long>(iso::GN_PARTS, std::max<long long>(1, (3ll * M * P / 4 + iso::GN_THREADS - 1) / iso::GN_THREADS));
+        hipLaunchKernelGGL(iso::gaussian_norm_kernel, dim3(parts), dim3(iso::GN_THREADS), 0, s, a, part);
+        ISR_LAUNCH_CHECK("iso_gaussian_grad_norm");
+    }
+    hipLaunchKernelGGL(iso::grad_norm_finish_kernel<2>, dim3(1), dim3(iso::GN_THREADS), 0, s, part, parts, max_norm, out);
+    ISR_LAUNCH_CHECK("iso_gaussian_grad_norm");
     return ISR_OK;
 }
 

@@ -243,8 +243,8 @@ Tensor rows8_read(const Tensor& codes, const Tensor& scales, const OptTensor& in
 // one stretch of memory, each element once (in any order of the dimensions)
 bool is_dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
 
-// the norm of all elements together [, and the tensors scaled in place]: out[0]
-Tensor grad_norm(const std::vector<Tensor>& tensors, double norm_type, double max_norm, bool clip) {
+// (norm, factor) of all elements together [, and the tensors scaled in place]
+Tensor norm_and_factor(const std::vector<Tensor>& tensors, double norm_type, double max_norm, bool clip) {
     const char* what = clip ? "clip_grads_" : "grad_norm";
     const int kind = norm_type == 2.0 ? 2 : norm_type == 1.0 ? 1 : norm_type == std::numeric_limits<double>::infinity() ? 0 : -1;
     TORCH_CHECK_VALUE(kind >= 0, what, ": norm_type must be 1, 2 or inf, not ", norm_type);
@@ -282,8 +282,10 @@ Tensor grad_norm(const std::vector<Tensor>& tensors, double norm_type, double ma
         for (const Tensor& t : tensors) t.unsafeGetTensorImpl()->bump_version();
         for (const auto& [i, c] : copies) tensors[i].copy_(c);
     }
-    return out[0];
+    return out;
 }
+Tensor grad_norm(const std::vector<Tensor>& tensors, double norm_type, double max_norm, bool clip) { return norm_and_factor(tensors, norm_type, max_norm, clip)[0]; }
+Tensor grad_norm_coef(const std::vector<Tensor>& tensors, double norm_type, double max_norm) { return norm_and_factor(tensors, norm_type, max_norm, false); }
 
 }  // namespace
 
@@ -301,4 +303,5 @@ void bind_rows(pybind11::module_& m) {
     m.def("rows8_write", &rows8_write);
     m.def("rows8_read", &rows8_read);
     m.def("grad_norm", &grad_norm);
+    m.def("grad_norm_coef", &grad_norm_coef);
 }

@@ -29,6 +29,7 @@ from . import scenes
 from .contrastive import contrastive_loss, contrastive_loss_batch, gather_rows, row_normalize, row_normalize_chain
 from .dist_utils import (allreduce_bucket, allreduce_grads, allreduce_grads_async, allreduce_rows_async, row_ranges, view_for,
                          wait_all)
+from .optim import check_max_norm, clip_grad_norm_
 from .rasterizer import DeferredFeatureRows
 from .render import prefetch, render
 from .rows import QuantizedRows
@@ -161,8 +162,11 @@ class SegTrainer:
     def __init__(self, scene: scenes.Scene, cameras: List[scenes.Camera], device="cuda", sample_batchsize=8192,
                  n_labels=64, lambda_sv=1e-6, lambda_mv=1e-6, lambda_3d=2.5e-6, sample_mv_frames=5, use_class_feat=False,
                  multiview=False, seed=0, rank=0, world=1, prefetch_geometry=None, fused_update=None, sampled_path=True,
-                 fused_tail=None, batched_losses=None, spatial_sort=True, fused_sampling=None):
+                 fused_tail=None, batched_losses=None, spatial_sort=True, fused_sampling=None, max_grad_norm=None):
+        """``max_grad_norm``: clip the (summed) gradient of ``_seg_feature`` to this 2-norm in every step; the norm of the last one is in
+        ``last_grad_norm`` (a scalar on the device)."""
         self.device = torch.device(device)
+        self.max_grad_norm = None if max_grad_norm is None else check_max_norm("SegTrainer", max_grad_norm)
         # Gaussians stored in Z-order of their centres (once, here): neighbours in memory are neighbours on screen, which
         # the binning kernels' workgroup-level counter merging and every per-Gaussian gather rely on.  A pure relabelling
         # of rows: `self.order[k]` is the caller's index of row k (see `features_in_input_order`).
@@ -534,10 +538,12 @@ class SegTrainer:
             if self.world == 1 and not self.split_tail:
                 if gate_ev is not None:
                     torch.cuda.current_stream(self.device).wait_event(gate_ev)
-                self.opt.step_rows(sink.rows, row_grads=sink.row_grads, dense=sink.dense)
+                self.opt.step_rows(sink.rows, row_grads=sink.row_grads, dense=sink.dense, max_grad_norm=self.max_grad_norm)
                 m._seg_cache = None
                 return loss.detach()
             if self.sharded_tail and m._seg_feature.shape[0] % self.world == 0:
+                if self.max_grad_norm is not None:
+                    raise RuntimeError("SegTrainer: max_grad_norm is not supported by the sharded tail (no rank has the whole gradient)")
                 self._tail_sharded(sink)
             elif self.exchange in ("peer", "peer_compact") and self.world > 1 and self.device.type == "cuda":
                 self._tail_with_peer_exchange(sink)
@@ -550,10 +556,21 @@ class SegTrainer:
             wait_all(allreduce_grads_async([m._seg_feature], self.world))
         else:
             allreduce_grads([m._seg_feature], self.world)
-        self.opt.step()
+        if self.max_grad_norm is None:
+            self.opt.step()
+        elif hasattr(self.opt, "clipped_step"):
+            self.opt.step(max_grad_norm=self.max_grad_norm)
+        else:
+            self._torch_grad_norm = clip_grad_norm_([m._seg_feature], self.max_grad_norm)
+            self.opt.step()
         self.opt.zero_grad(set_to_none=True)
         m._seg_cache = None          # the graph of this step is gone
         return loss.detach()
+
+    @property
+    def last_grad_norm(self):
+        """The gradient's norm before clipping, of the last step with ``max_grad_norm``."""
+        return getattr(self.opt, "last_grad_norm", None) if hasattr(self.opt, "clipped_step") else getattr(self, "_torch_grad_norm", None)
 
     # -- everything behind the blend through ONE C entry (isr_seg_step_tail) instead of the autograd graph -----------------
     def _c_tail_ok(self, it, merged, drawn, pkg) -> bool:
@@ -566,6 +583,8 @@ class SegTrainer:
                 and self.sampled_path and self.batched_losses and self.stacked_losses and self.device.type == "cuda"):
             return False
         if self.multiview and self.lmv > 0 and it % 10 == 0:
+            return False
+        if self.max_grad_norm is not None:         # the gradient's norm comes between the reduction and the step
             return False
         if self.l3d > 0 and drawn[3] is None:
             return False
@@ -758,9 +777,12 @@ class SegTrainer:
             self._peer.all_reduce_compact_(touched)
         else:
             self._peer.all_reduce_()
-        opt.begin_step()
-        opt.step_range(0, P)
-        opt.end_step()
+        if self.max_grad_norm is not None:
+            opt.clipped_step(self.max_grad_norm)
+        else:
+            opt.begin_step()
+            opt.step_range(0, P)
+            opt.end_step()
         p.grad = None
         # a wait that timed out only sets a status bit and lets the stream run on (a dead peer must not wedge the GPU): read the
         # word every `peer_check_every` steps (one blocking 4-byte read), so that replicas never diverge silently for long
@@ -795,6 +817,11 @@ class SegTrainer:
             works.append(allreduce_rows_async(p.grad, r0, r1, self.world))
         if timed:
             t_grads = ev(); t_grads.record()
+        coef = None
+        if self.max_grad_norm is not None:          # (the norm is the whole sum's: every range has to have arrived)
+            wait_all([w for w in works if w is not None])
+            works = [None] * len(works)
+            coef = opt._clip_coef([p.grad], self.max_grad_norm)
         opt.begin_step()
         for (r0, r1), w in zip(bounds, works):
             if timed:
@@ -803,7 +830,7 @@ class SegTrainer:
                 w.wait()                 # the compute stream waits for this range's collective; the host does not
             if timed:
                 b = ev(); b.record()
-            opt.step_range(r0, r1)
+            opt.step_range(r0, r1, coef=coef)
             if timed:
                 c = ev(); c.record()
                 marks.append((a, b, c))
@@ -984,12 +1011,15 @@ class RgbTrainer:
     lambda_normal*(1 - <rend_normal, surf_normal>) -> backward (full geometry gradients) -> Adam."""
 
     def __init__(self, scene, cameras, targets, device="cuda", lambda_dssim=0.2, lambda_normal=0.05, lambda_dist=0.0,
-                 rank=0, world=1, densify=None, scene_extent=None, spatial_sort=True, fused_update=None):
-        """``spatial_sort``: store the Gaussians in Z-order of their centres (a row permutation, once, here; rows that the
+                 rank=0, world=1, densify=None, scene_extent=None, spatial_sort=True, fused_update=None, max_grad_norm=None):
+        """``max_grad_norm``: clip the gradients of the six parameter groups together to this 2-norm in every step; the norm of the last one
+        is in ``last_grad_norm``.  ``spatial_sort``: store the Gaussians in Z-order of their centres (a row permutation, once, here; rows that the
         density control appends later go to the end).  ``densify``: None (off) or a dict overriding the reference's schedule (arguments/__init__.py:106-125):
         ``from_iter=500, until_iter=15000, interval=100, opacity_reset_interval=3000, grad_threshold=0.0002,
         opacity_cull=0.05, percent_dense=0.01``; ``scene_extent`` = the reference's ``cameras_extent``."""
         from .losses import l1_loss, photometric_loss, ssim, train_loss
+        self.max_grad_norm = None if max_grad_norm is None else check_max_norm("RgbTrainer", max_grad_norm)
+        self.last_grad_norm = None
         self.l1, self.ssim, self.photometric, self.train_loss = l1_loss, ssim, photometric_loss, train_loss
         self.device = torch.device(device)
         self.order = None
@@ -1080,6 +1110,8 @@ class RgbTrainer:
         is host-paced otherwise (0.78 ms of Python for 0.62 ms of kernels).  ISR_C_TAIL=0: always the autograd path."""
         if not (self.c_tail and self.fused_update and self.fused_loss and self.world == 1 and self.device.type == "cuda"):
             return False
+        if self.max_grad_norm is not None:         # the gradients' norm comes between the backward pass and the step
+            return False
         img = pkg["render"]
         n1 = getattr(img, "grad_fn", None)
         n2 = getattr(pkg["rend_normal"], "grad_fn", None)
@@ -1157,13 +1189,17 @@ class RgbTrainer:
             # one flat collective for all six groups' gradients (they are final only after the per-Gaussian backward pass)
             lv = self.opt.leaves
             self.opt.step(allreduce_bucket(self.opt.leaf_grads(), self.world,
-                                           like=[lv["xyz"], lv["shs"], lv["opacity"], lv["scaling"], lv["rotation"]]))
+                                           like=[lv["xyz"], lv["shs"], lv["opacity"], lv["scaling"], lv["rotation"]]),
+                          max_grad_norm=self.max_grad_norm)
+            self.last_grad_norm = self.opt.last_grad_norm
             self.opt.zero_grad(set_to_none=True)
             return loss.detach(), pkg
         pkg = render(self.cams[vi], self.model, self.pipe, self.bg)
         loss = self._loss(pkg, vi)
         loss.backward()
         allreduce_grads([p for gr in self.opt.param_groups for p in gr["params"]], self.world)
+        if self.max_grad_norm is not None:
+            self.last_grad_norm = clip_grad_norm_([p for gr in self.opt.param_groups for p in gr["params"]], self.max_grad_norm)
         if self.densify_cfg is not None:
             self._density_control(it + 1, pkg)          # the reference counts iterations from 1
         self.opt.step()

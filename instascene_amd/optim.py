@@ -53,6 +53,7 @@ class GaussianAdam:
         self.exp_avg = {g: torch.zeros_like(getattr(model, _ATTR[g])) for g in GROUPS}
         self.exp_avg_sq = {g: torch.zeros_like(getattr(model, _ATTR[g])) for g in GROUPS}
         self.step_count = 0
+        self.last_grad_norm = None      # of the last step with max_grad_norm: a float32 scalar on the device
         self._acts = None               # activations of the current parameters, written by the last step
         self.leaves = None
 
@@ -60,7 +61,24 @@ class GaussianAdam:
     def _params(self):
         return [getattr(self.model, _ATTR[g]) for g in GROUPS]
 
-    def _launch(self, grads, want_acts: bool):
+    def _clip_coef(self, grads, max_grad_norm: float):
+        """``min(1, max_grad_norm / (norm + 1e-6))`` of the raw parameters' gradients (``iso_gaussian_grad_norm``: this optimiser's chain rule on
+        the way), on the device; the norm goes to ``last_grad_norm``."""
+        ps = self._params()
+        dev = ps[0].device
+        g = [None if t is None else t.contiguous().float() for t in grads]
+        L = lib()
+        nbytes = L.iso_grad_norm_scratch_bytes(1, None)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        out = torch.empty(2, dtype=torch.float32, device=dev)
+        p = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
+        with _hot.on_device(dev):
+            check(L.iso_gaussian_grad_norm(ps[0].shape[0], 1 + ps[2].shape[1], _table([t.data for t in ps]), p(g[0]), p(g[1]), p(g[2]), p(g[3]),
+                                           p(g[4]), float(max_grad_norm), p(out), p(scratch), nbytes, _hot.stream_ptr(dev)), "iso_gaussian_grad_norm")
+        self.last_grad_norm = out[0]
+        return out[1:2]
+
+    def _launch(self, grads, want_acts: bool, coef=None):
         ps = self._params()
         P = ps[0].shape[0]
         M = 1 + ps[2].shape[1]
@@ -73,11 +91,11 @@ class GaussianAdam:
         p = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
         g = [None if t is None else t.contiguous().float() for t in grads]
         with _hot.on_device(dev):
-            check(lib().iso_gaussian_adam_step(
+            check(lib().iso_gaussian_adam_step_clipped(
                 P, M, _table([t.data for t in ps]), _table([self.exp_avg[k] for k in GROUPS]),
                 _table([self.exp_avg_sq[k] for k in GROUPS]), lr, float(self.betas[0]), float(self.betas[1]), self.eps,
                 max(1, self.step_count), p(g[0]), p(g[1]), p(g[2]), p(g[3]), p(g[4]),
-                *(p(a) for a in (acts if acts is not None else (None,) * 4)),
+                *(p(a) for a in (acts if acts is not None else (None,) * 4)), p(coef),
                 _hot.stream_ptr(dev)), "iso_gaussian_adam_step")
         return acts
 
@@ -97,13 +115,16 @@ class GaussianAdam:
         lv = self.leaves
         return [lv["xyz"].grad, lv["shs"].grad, lv["opacity"].grad, lv["scaling"].grad, lv["rotation"].grad]
 
-    def step(self, grads=None):
-        """Chain rule + Adam + the next activations from the leaves' gradients (or ``grads``, e.g. their sum over ranks)."""
+    def step(self, grads=None, max_grad_norm: Optional[float] = None):
+        """Chain rule + Adam + the next activations from the leaves' gradients (or ``grads``, e.g. their sum over ranks).
+        ``max_grad_norm``: the gradients of the six raw parameters clipped to this global norm, as ``clip_grad_norm_`` in front of
+        ``torch.optim.Adam`` would - the factor is applied inside the step's kernel; their norm is then in ``last_grad_norm``."""
         if self.leaves is None:
             raise RuntimeError("GaussianAdam.step: begin() was not called")
         grads = self.leaf_grads() if grads is None else grads
+        coef = None if max_grad_norm is None else self._clip_coef(grads, check_max_norm("GaussianAdam.step", max_grad_norm))
         self.step_count += 1
-        acts = self._launch(grads, want_acts=True)
+        acts = self._launch(grads, want_acts=True, coef=coef)
         ps = self._params()
         for prm in ps:
             torch.autograd.graph.increment_version(prm)         # the kernel wrote through raw pointers
@@ -138,6 +159,20 @@ class GaussianAdam:
 
 
 # -- the global norm of many gradients, and clipping ----------------------------------------------------------------------------
+def check_max_norm(what: str, max_norm) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"{what}: the largest norm must not be negative, is {max_norm}")
+    return max_norm
+
+
+def norm_and_coef(tensors: Sequence[torch.Tensor], max_norm: float):
+    """``(norm, coef)`` of gradients that an optimiser kernel will scale itself (``FeatureAdam``): one-element views of one tensor;
+    ``coef = min(1, max_norm / (norm + 1e-6))``.  Nothing is written to the gradients."""
+    out = _ext().grad_norm_coef(list(tensors), 2.0, max_norm)
+    return out[0], out[1:2]
+
+
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """The norm (2, 1 or inf) of all elements of ``tensors`` together, as a float32 scalar on their device; nothing is synchronised.
     float32, bfloat16 and float16 may be mixed; sums are held in 64 bits.  No tensors: 0."""
@@ -153,9 +188,7 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
     read once and not written.  Two of them may not share memory.  ``error_if_nonfinite`` reads the norm back (a synchronisation) and
     raises before anything is scaled."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    max_norm = float(max_norm)
-    if not max_norm >= 0.0:
-        raise ValueError(f"clip_grads_: max_norm must not be negative, is {max_norm}")
+    max_norm = check_max_norm("clip_grads_", max_norm)
     if not grads:
         return torch.tensor(0.0)
     if error_if_nonfinite:

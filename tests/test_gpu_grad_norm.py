@@ -189,3 +189,143 @@ def test_refusals_on_the_device():
                         (lambda: clip_grads_([x], float("nan")), ValueError), (lambda: grad_norm([x.to_sparse()]), RuntimeError)]:
         with pytest.raises(error):
             call()
+
+
+# ---- in the optimisers and trainers -----------------------------------------------------------------------------------------------------
+def _gaussians(P, M, seed):
+    """A model's raw parameters, and gradients of its activated tensors."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")
+
+    class Model:
+        pass
+
+    m = Model()
+    mk = lambda t: torch.nn.Parameter(t)
+    m._xyz, m._features_dc, m._features_rest = mk(n(P, 3)), mk(n(P, 1, 3)), mk(n(P, M - 1, 3))
+    m._opacity, m._scaling, m._rotation = mk(n(P, 1)), mk(0.5 * n(P, 2) - 3), mk(n(P, 4))
+    return m, [n(P, 3) * 1e-2, n(P, M, 3) * 1e-3, n(P, 1) * 1e-2, n(P, 2), n(P, 4) * 1e-2]
+
+
+@pytest.mark.parametrize("P,M", [(1, 16), (37, 16), (5003, 4), (40001, 16), (300, 1)])
+@pytest.mark.parametrize("missing", [(), (1, 3)])
+def test_gaussian_adam_clips_the_raw_gradients(P, M, missing):
+    from instascene_amd.optim import GaussianAdam
+    lrs = dict(xyz=1e-3, f_dc=2e-3, f_rest=1e-4, opacity=5e-2, scaling=5e-3, rotation=1e-3)
+    m, grads = _gaussians(P, M, 3)
+    grads = [None if i in missing else t for i, t in enumerate(grads)]
+    # raw gradients in 64 bits through the activations
+    raw = [getattr(m, k).detach().double().requires_grad_(True) for k in ("_xyz", "_features_dc", "_features_rest", "_opacity", "_scaling", "_rotation")]
+    acts = [raw[0], torch.cat((raw[1], raw[2]), 1), torch.sigmoid(raw[3]), torch.exp(raw[4]), torch.nn.functional.normalize(raw[5])]
+    value = sum((a * t.double()).sum() for a, t in zip(acts, grads) if t is not None)
+    value.backward()
+    norm = math.sqrt(sum(float(r.grad.square().sum()) for r in raw if r.grad is not None))
+    start = {k: getattr(m, k).detach().clone() for k in ("_xyz", "_features_dc", "_features_rest", "_opacity", "_scaling", "_rotation")}
+    opt = GaussianAdam(m, lrs)
+    opt.begin()
+    opt.step(grads, max_grad_norm=0.25 * norm)
+    # the 32-bit chain rule: at most 12 roundings and an expf (2 u) per gradient, i.e. below 20 u of the norm
+    assert abs(float(opt.last_grad_norm) - norm) <= 20 * U * norm + 1e-30
+    # a first step of Adam from clipped gradients g: m = 0.1 g, v = 0.001 g^2
+    coef = 0.25 * norm / (norm + 1e-6)
+    for name, r in zip(("xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation"), raw):
+        if r.grad is None or r.numel() == 0:
+            assert torch.equal(opt.exp_avg[name], torch.zeros_like(opt.exp_avg[name]))
+            continue
+        # (a rotation's gradient cancels: the noise is that of its terms, below the row's largest)
+        big = r.grad.abs().reshape(P, -1).amax(1).reshape(-1, *([1] * (r.grad.dim() - 1))) + (grads[4].double().abs().amax(1, keepdim=True) * 4 if name == "rotation" else 0.0)
+        assert bool(((opt.exp_avg[name].double() - 0.1 * coef * r.grad).abs() <= 0.1 * coef * 64 * U * big + 1e-30).all()), name
+    # a bound that does not bind: the same step as without one
+    n, gr = _gaussians(P, M, 3)
+    o, (k, _) = GaussianAdam(n, lrs), _gaussians(P, M, 3)
+    q = GaussianAdam(k, lrs)
+    gr = [None if i in missing else t for i, t in enumerate(gr)]
+    for a, kw in ((o, {}), (q, {"max_grad_norm": 1e9})):
+        a.begin()
+        a.step(gr, **kw)
+    for name in start:
+        assert torch.equal(getattr(n, name), getattr(k, name))
+
+
+@pytest.mark.parametrize("P,F", [(1, 4), (1001, 32), (20000, 64), (33, 256)])
+def test_feature_adam_clips(P, F):
+    """FeatureAdam.step(max_grad_norm) = clip_grad_norm_ then FeatureAdam.step, bit for bit; the gradient itself stays."""
+    from instascene_amd.contrastive import FeatureAdam
+    g = torch.Generator(device="cuda").manual_seed(P)
+    start, grads = torch.randn(P, F, generator=g, device="cuda"), [torch.randn(P, F, generator=g, device="cuda") for _ in range(3)]
+    a, b = torch.nn.Parameter(start.clone()), torch.nn.Parameter(start.clone())
+    oa, ob = FeatureAdam(a, 0.01), FeatureAdam(b, 0.01)
+    for t in grads:
+        bound = 0.5 * float(t.norm())
+        a.grad, b.grad = t.clone(), t.clone()
+        oa.step(max_grad_norm=bound)
+        n = clip_grad_norm_([b], bound)
+        ob.step()
+        assert torch.equal(a, b) and torch.equal(a.grad, t) and float(n) == float(oa.last_grad_norm)
+    with pytest.raises(ValueError):
+        oa.step(max_grad_norm=-1.0)
+
+
+def _seg(**kw):
+    from instascene_amd import scenes
+    from instascene_amd.harness import SegTrainer
+    sc = scenes.synthetic_scene(4000, 16, 5, math.log(0.04))
+    return SegTrainer(sc, scenes.ring_cameras(6, 128, 96), device="cuda", sample_batchsize=2048, n_labels=12, use_class_feat=True, seed=3, **kw)
+
+
+def test_trainers_clip():
+    """SegTrainer / RgbTrainer(max_grad_norm): a bound that does not bind changes nothing, one that does gives the moments of clipped
+    gradients - on every path of the step (one C entry, autograd, split tail, torch's optimiser)."""
+    from instascene_amd import rasterizer as rz, scenes
+    from instascene_amd.harness import RgbTrainer
+    rz.set_mode("exact")
+    rz.set_tracer(False)
+    try:
+        plain, wide = _seg(), _seg(max_grad_norm=1e9)
+        for it in range(3):
+            plain.step(it)
+            wide.step(it)
+        assert torch.equal(plain.model._seg_feature, wide.model._seg_feature)
+        norm = float(_first_norm(_seg(max_grad_norm=1e9)))
+        assert norm > 0
+        results = []
+        for kw, tweak in (({}, None), ({}, "split_tail"), ({"fused_tail": False}, None), ({"fused_update": False, "fused_tail": False}, None)):
+            t = _seg(max_grad_norm=0.1 * norm, **kw)
+            if tweak:
+                setattr(t, tweak, True)
+            t.step(0)
+            assert abs(float(t.last_grad_norm) - norm) <= 1e-5 * norm           # (the paths sum the rows in different orders)
+            avg = t.opt.exp_avg if hasattr(t.opt, "exp_avg") else t.opt.state[t.model._seg_feature]["exp_avg"]
+            # the first moment is 0.1 of the clipped gradient; the factor is 0.1 norm / (norm + 1e-6), with a norm of 1e-4 here 0.8 % below 0.1
+            want = 0.1 * norm * (0.1 * norm / (norm + 1e-6))
+            assert abs(float(avg.norm()) - want) <= 1e-4 * want
+            results.append(avg.clone())
+        for r in results[1:]:
+            assert float((r - results[0]).norm()) <= 1e-4 * float(results[0].norm())
+        sc = scenes.synthetic_scene(3000, 4, 7, math.log(0.05))
+        cams = scenes.ring_cameras(4, 96, 64)
+        targets = [torch.rand(3, 64, 96, generator=torch.Generator().manual_seed(k)) for k in range(4)]
+        mk = lambda **kw: RgbTrainer(sc, cams, targets, device="cuda", **kw)
+        plain, wide = mk(), mk(max_grad_norm=1e9)
+        for it in range(2):
+            plain.step(it)
+            wide.step(it)
+        for k in ("_xyz", "_features_dc", "_features_rest", "_opacity", "_scaling", "_rotation"):
+            assert torch.equal(getattr(plain.model, k), getattr(wide.model, k)), k
+        a, b = mk(max_grad_norm=1e-4), mk(max_grad_norm=1e-4, fused_update=False)
+        a.step(0)
+        b.step(0)
+        assert float(a.last_grad_norm) > 1e-4
+        assert abs(float(a.last_grad_norm) - float(b.last_grad_norm)) <= 1e-4 * float(b.last_grad_norm)
+        for name, p in (("xyz", b.model._xyz), ("scaling", b.model._scaling), ("rotation", b.model._rotation), ("f_rest", b.model._features_rest)):
+            want = b.opt.state[p]["exp_avg"]
+            assert float((a.opt.exp_avg[name] - want).norm()) <= 1e-3 * float(want.norm())
+        with pytest.raises(ValueError):
+            _seg(max_grad_norm=-1.0)
+    finally:
+        rz.set_tracer(True)
+
+
+def _first_norm(t):
+    t.step(0)
+    return t.last_grad_norm

@@ -475,3 +475,50 @@ def test_a_trained_table_in_8_bits_renders(code, group):
               + 2.0 ** -10 * rows.double().abs().amax(1, keepdim=True) / 448 + 4 * U, "codes")
         with pytest.raises(RuntimeError):
             m.compact_features()
+
+
+def test_a_residual_table_is_trained_clipped_and_put_away():
+    """All of it together, as a program uses it: a frozen base table and a trained one, rms_norm of their sum with a learned gain, the
+    contrastive loss on gathered rows, the gradients clipped together, the steps; then the trained rows in 8 bits and read back by index.
+    Every piece against the same step in 64 bits."""
+    from instascene_amd.contrastive import contrastive_loss
+    from instascene_amd.optim import clip_grad_norm_
+    P, F, n = 3000, 32, 1024
+    base = make((P, F), F32, 1)
+    delta = torch.nn.Parameter(0.1 * make((P, F), F32, 2))
+    gain = torch.nn.Parameter(1.0 + 0.1 * make((F,), F32, 3))
+    labels = torch.randint(1, 9, (P,), device="cuda")
+    opt = torch.optim.SGD([delta, gain], lr=1.0)
+    for step in range(3):
+        pick = torch.randint(0, P, (n,), device="cuda")
+        opt.zero_grad()
+        y, s = rms_norm(delta, gain, 1e-6, residual=base)
+        (contrastive_loss(y[pick], labels[pick], num_labels=9) + 1e-3 * s.square().sum()).backward()
+        with torch.enable_grad():
+            d64, g64 = delta.detach().double().requires_grad_(True), gain.detach().double().requires_grad_(True)
+            s64 = d64 + base.double()
+            y64 = s64 / torch.sqrt(s64.square().mean(1, keepdim=True) + 1e-6) * g64
+            leaf = y.detach()[pick].requires_grad_(True)                   # the loss' own gradient at y
+            gl, = torch.autograd.grad(contrastive_loss(leaf, labels[pick], num_labels=9), leaf)
+            gy = torch.zeros(P, F, dtype=torch.float64, device="cuda").index_add_(0, pick, gl.double())
+            want = torch.autograd.grad((y64 * gy).sum() + 1e-3 * s64.square().sum(), (d64, g64))
+        norm = math.sqrt(sum(float(w.square().sum()) for w in want))
+        before = delta.detach().clone()
+        got = clip_grad_norm_([delta, gain], 0.5 * norm)
+        assert abs(float(got) - norm) <= 1e-5 * norm
+        coef = 0.5 * norm / (norm + 1e-6)
+        for p, w in ((delta, want[0]), (gain, want[1])):
+            assert float((p.grad.double() - coef * w).norm()) <= 1e-5 * float((coef * w).norm())
+        opt.step()
+        assert torch.equal(delta, before - delta.grad)
+    with torch.no_grad():
+        q, s = rms_norm_quantized(delta, gain, 1e-6, residual=base, dtype=torch.int8)
+        y = rms_norm(delta, gain, 1e-6, residual=base)[0]
+        top = y.abs().amax(1, keepdim=True)
+        check(q.read(), y.double(), top.double() * (0.5 / 127 + 60 * U), "8 bits")        # half a step of the row's largest / 127
+        table = QuantizedRows(P, F, dtype=torch.int8)
+        order = torch.randperm(P, device="cuda")
+        table.write(y[order], order)
+        check(table.read(), y.double(), top.double() * (0.5 / 127 + 60 * U), "written by index")
+        assert torch.equal(gather_rows(table, order[:n]), table.read()[order[:n]])
+        check(gather_rows(table, order[:n]).norm(dim=1), y[order[:n]].double().norm(dim=1), top[order[:n], 0].double() * math.sqrt(F) * 0.6 / 127, "lengths")
