@@ -19,28 +19,34 @@ bool code_type(int c) { return c == iso::CODE_INT8 || c == iso::CODE_E4M3; }
 bool group_ok(int F, int group) { return group == F || ((group == 32 || group == 64 || group == 128) && F % group == 0); }
 int group_shift(int F, int group) { return group == F ? 31 : group == 32 ? 5 : group == 64 ? 6 : 7; }
 
-// From this many bytes a stream is read (backward pass, 8-bit writes) or written (backward pass, 8-bit reads) past the caches: half of the
-// 256 MB last-level cache, so that it would push out more than the next kernel finds of it.  Measured on 1.28 GB / 134 MB streams: the whole
-// 8-bit table written and read 550 -> 530 us, rms_norm_quantized of [16384, 4096] bfloat16 94 -> 86, the backward pass of [8192, 8192] bfloat16
-// 149 -> 106, of [1.5 M, 32] float32 165 -> 132; a forward pass, whose outputs the next kernel reads, loses (128 -> 134) and keeps its lines.
-constexpr long long NT_BYTES = 128ll << 20;
+// From this many bytes on a stream goes past the caches (256 MB in front of the memory), from which the next kernel would find little:
+// the backward pass reads and writes so (forward + backward per stream of 32 / 48 / 64 / 96 MB: [n, 32] float32 47.2 / 65.8 / 89.3 / 134 us, with
+// cached lines 44.6 / 71.5 / 95.4 / 147; [n, 4096] bfloat16 56.5 / 79.6 / 107 / 157, cached 51.6 / 74.9 / 110 / 176), 8-bit rows are written from and
+// read to (the table of [5 M, 64] 530 us, cached 550; [16384, 4096] bfloat16 quantised 86, cached 94; at 92 MB 61 and 68 with 40 and 46 at 64 MB the
+// other way round).  A forward pass, whose outputs the next kernel reads, loses (128 -> 134) and keeps its lines.
+constexpr long long NT_BACKWARD = 64ll << 20, NT_CODES = 128ll << 20;
 
-// threads per row (1 << tsh) and vectors per thread for a row of `vecs` vectors; 0 vectors per thread: the *_long form.
-// Within a wave `least` vectors per thread where there are rows enough to fill the chip all the same: 2 for 8-bit rows, whose work per row
-// (scales, the norm) weighs less then ([5 M, 64]: written 283 -> 258 us, read 359 -> 252; 4 are slower again, 64-byte pieces), 1 for the norm
-// ([1.5 M, 32]: 128 us, 160 with 2).  Beyond a wave 2 per thread ([8192, 8192] bfloat16: 240 us forward and backward, 333 with 4, 456 with 8).
-// Where there are so few rows that the chip would stand idle, up to 512 threads.
-void row_shape(int vecs, long long rows, int least, int max_nv, int& tsh, int& nv) {
-    tsh = 0;
+// How a kernel lays rows of `vecs` vectors over its threads: tpr threads and nv vectors per thread for each (nv = 0: the *_long form), thread t of
+// the row = threadIdx.x & mask, row of the workgroup = threadIdx.x >> tsh, rpb rows per workgroup.
+// Up to a wave: a power of two, `least` vectors per thread where there are rows enough to fill the chip all the same: 2 for 8-bit rows, whose work
+// per row (scales, the norm) weighs less then ([5 M, 64]: written 283 -> 258 us, read 359 -> 252; 4 are slower again, 64-byte pieces), 1 for the
+// norm ([1.5 M, 32]: 128 us, 160 with 2).  Beyond: a workgroup of whole waves per row, 2 vectors per thread ([8192, 8192] bfloat16: 240 us forward
+// and backward, 333 with 4, 456 with 8), as many waves as the row needs.  Where there are so few rows that the chip would stand idle, 1 vector
+// per thread.
+struct RowShape { int tpr, mask, tsh, rpb, nv, block; };
+RowShape row_shape(int vecs, long long rows, int least, int max_nv) {
+    int tsh = 0;
     while ((1 << tsh) < vecs && tsh < 6) tsh++;
     while (tsh > 0 && (vecs + (1 << (tsh - 1)) - 1) >> (tsh - 1) <= least && (rows << (tsh - 1)) >= 2048 * 256) tsh--;
-    while (tsh >= 6 && tsh < 9 && (1 << tsh) < vecs && ((vecs + (1 << tsh) - 1) >> tsh > 2 || (rows << tsh) < 256 * 256)) tsh++;
-    const int need = (vecs + (1 << tsh) - 1) >> tsh;
-    nv = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : need <= 8 ? 8 : 0;
-    if (nv > max_nv) nv = 0;
-    if (nv == 0) tsh = 9;
+    const int per_lane = (vecs + (1 << tsh) - 1) >> tsh;
+    if (per_lane <= (tsh == 6 && rows * 64 < 256 * 256 ? 1 : 2)) return {1 << tsh, (1 << tsh) - 1, tsh, 256 >> tsh, per_lane, 256};
+    for (int nv = rows * ((vecs + 1) / 2) < 256 * 256 ? 1 : 2; nv <= max_nv; nv *= 2) {
+        const int waves = (vecs + 64 * nv - 1) / (64 * nv);
+        if (waves <= 8) return {64 * waves, 0x7fffffff, 31, 1, nv, 64 * waves};
+    }
+    return {512, 0x7fffffff, 31, 1, 0, 512};
 }
-int row_block(int tsh) { return tsh > 6 ? 1 << tsh : 256; }         // beyond a wave a workgroup is one row
+template <class A> void set_shape(A& a, const RowShape& r) { a.tpr = r.tpr; a.mask = r.mask; a.tsh = r.tsh; a.rpb = r.rpb; }
 
 #define ROWS_NV(nv, even, call, call_long) \
     do { if (nv == 1) { if (even) { call(1, true); } else { call(1, false); } } else if (nv == 2) { if (even) { call(2, true); } else { call(2, false); } } \
@@ -49,11 +55,12 @@ int row_block(int tsh) { return tsh > 6 ? 1 << tsh : 256; }         // beyond a 
 
 template <class T, int OUT> void launch_forward(iso::RmsArgs a, hipStream_t s) {
     constexpr int N = iso::RowVec<T>::N;
-    int nv;
-    row_shape((a.F + N - 1) / N, a.rows, OUT == 0 ? 1 : 2, 8, a.tsh, nv);
-    a.tpr = 1 << a.tsh;
-    const bool nt = OUT != 0 && a.rows * a.F * (long long)sizeof(T) >= NT_BYTES, even = a.F % N == 0;
-    const int block = row_block(a.tsh), rpb = block >> a.tsh;
+    const RowShape sh = row_shape((a.F + N - 1) / N, a.rows, OUT == 0 ? 1 : 2, 8);
+    set_shape(a, sh);
+    const int nv = sh.nv;
+    // (past the caches only whole 128-byte lines per load: [8 M, 32] float32 224 us so with 4 threads per row, 174 cached)
+    const bool nt = OUT != 0 && a.tpr >= 8 && a.rows * a.F * (long long)sizeof(T) >= NT_CODES, even = a.F % N == 0;
+    const int block = sh.block, rpb = sh.rpb;
     const long long step = MAX_THREADS / block * rpb;
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
@@ -76,20 +83,17 @@ void launch_codes(int code, int type, const iso::RmsArgs& a, hipStream_t s) {
     else launch_forward_type<iso::CODE_E4M3>(type, a, s);
 }
 
-// workgroups of the backward pass = partial rows of dw: enough to fill the chip, few enough that the partials stay small against the rows
-template <class T> void backward_shape(long long rows, int F, int& tsh, int& nv, int& block, int& grid) {
-    row_shape((F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, rows, 1, 4, tsh, nv);
-    block = row_block(tsh);
-    if (nv == 0) { grid = (int)std::min<long long>(64, std::max<long long>(1, rows)); return; }       // slices of the columns' sums
-    const int rpb = block >> tsh;
-    const long long need = (rows + rpb - 1) / rpb;
-    const long long most = std::max<long long>(512, std::min<long long>(2048, (1 << 20) / F));
+// workgroups of the backward pass = partial rows of dw: enough to keep the memory busy (two of 256 threads per compute unit do for wide rows:
+// 768 and 1024 workgroups took 1 to 14 % longer at [n, 2048..4096] float32), few enough that the partials stay small against the rows
+template <class T> RowShape backward_shape(long long rows, int F, int& grid) {
+    const RowShape sh = row_shape((F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, rows, 1, 4);
+    if (sh.nv == 0) { grid = (int)std::min<long long>(64, std::max<long long>(1, rows)); return sh; }       // slices of the columns' sums
+    const long long need = (rows + sh.rpb - 1) / sh.rpb, most = std::max<long long>(512, std::min<long long>(2048, (1 << 20) / F));
     grid = (int)std::max<long long>(1, std::min(need, most));
+    return sh;
 }
-void backward_shape_type(int type, long long rows, int F, int& tsh, int& nv, int& block, int& grid) {
-    if (type == 0) backward_shape<float>(rows, F, tsh, nv, block, grid);
-    else if (type == 1) backward_shape<__bf16>(rows, F, tsh, nv, block, grid);
-    else backward_shape<_Float16>(rows, F, tsh, nv, block, grid);
+RowShape backward_shape_type(int type, long long rows, int F, int& grid) {
+    return type == 0 ? backward_shape<float>(rows, F, grid) : type == 1 ? backward_shape<__bf16>(rows, F, grid) : backward_shape<_Float16>(rows, F, grid);
 }
 template <class T, bool EVEN, bool NT> void launch_backward_nv(const iso::RmsBackArgs& a, int nv, int block, int grid, hipStream_t s) {
     if (nv == 1) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 1, EVEN, NT>), dim3(grid), dim3(block), 0, s, a);
@@ -98,7 +102,7 @@ template <class T, bool EVEN, bool NT> void launch_backward_nv(const iso::RmsBac
 }
 template <class T> void launch_backward(iso::RmsBackArgs a, int nv, int block, int grid, hipStream_t s) {
     if (nv != 0) {
-        const bool even = a.F % iso::RowVec<T>::N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= NT_BYTES;
+        const bool even = a.F % iso::RowVec<T>::N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= NT_BACKWARD;
         if (even && nt) launch_backward_nv<T, true, true>(a, nv, block, grid, s);
         else if (even) launch_backward_nv<T, true, false>(a, nv, block, grid, s);
         else if (nt) launch_backward_nv<T, false, true>(a, nv, block, grid, s);
@@ -112,11 +116,11 @@ template <class T> void launch_backward(iso::RmsBackArgs a, int nv, int block, i
 }
 template <class T, int CODE> void launch_read(iso::ReadArgs a, hipStream_t s) {
     constexpr int N = iso::RowVec<T>::N;
-    int nv;
-    row_shape((a.F + N - 1) / N, a.rows, 2, 8, a.tsh, nv);
-    a.tpr = 1 << a.tsh;
-    const bool even = a.F % N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= NT_BYTES;
-    const int block = row_block(a.tsh), rpb = block >> a.tsh;
+    const RowShape sh = row_shape((a.F + N - 1) / N, a.rows, 2, 8);
+    set_shape(a, sh);
+    const int nv = sh.nv;
+    const bool even = a.F % N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= NT_CODES;
+    const int block = sh.block, rpb = sh.rpb;
     const long long step = MAX_THREADS / block * rpb;
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
@@ -178,8 +182,8 @@ int iso_rms_norm_quant(int type, int code, long long rows, int F, int group, con
 
 size_t iso_rms_norm_scratch_bytes(int type, long long rows, int F) {
     if (!row_type(type) || rows <= 0 || F < 1 || F > (1 << 24)) return 0;
-    int tsh, nv, block, grid;
-    backward_shape_type(type, rows, F, tsh, nv, block, grid);
+    int grid;
+    backward_shape_type(type, rows, F, grid);
     return (size_t)grid * (size_t)F * sizeof(float);
 }
 
@@ -195,9 +199,10 @@ int iso_rms_norm_backward(int type, long long rows, int F, const void* x, long l
     iso::RmsBackArgs a = {};
     a.rows = rows; a.F = F; a.w32 = weight_is_float; a.x = x; a.ldx = x_stride; a.res = residual; a.ldr = residual_stride; a.w = weight; a.rstd = rstd;
     a.gy = gy; a.ldg = gy_stride; a.gs = gs; a.ldgs = gs_stride; a.ds = ds; a.dw_part = dw ? (float*)scratch : nullptr;
-    int nv, block, grid;
-    backward_shape_type(type, rows, F, a.tsh, nv, block, grid);
-    a.tpr = 1 << a.tsh;
+    int grid;
+    const RowShape sh = backward_shape_type(type, rows, F, grid);
+    set_shape(a, sh);
+    const int nv = sh.nv, block = sh.block;
     if (type == 0) launch_backward<float>(a, nv, block, grid, s);
     else if (type == 1) launch_backward<__bf16>(a, nv, block, grid, s);
     else launch_backward<_Float16>(a, nv, block, grid, s);
