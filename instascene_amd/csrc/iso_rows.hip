@@ -23,80 +23,105 @@ template <class T> struct RowVec { static constexpr int N = 16 / (int)sizeof(T);
 // (alignment of one element: rows of odd widths and views of buckets start anywhere; gfx950 loads unaligned vectors)
 template <class T, int N> struct Unaligned { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
 
-// Sixteen bytes of a row as they lie in memory, zeros beyond its F elements and for rows that are off.  EVEN: F is a multiple of the
-// vector, so a vector lies in the row or behind it: the address is drawn back into the row and the value dropped, without a branch.
-// NT: past the caches (a stream that is longer than they are and not read again).
-template <class T, int N, bool EVEN, bool NT = false> __device__ __forceinline__ typename Unaligned<T, N>::type raw_load(const T* row, int at, int F, bool on) {
+// ---- sixteen bytes of a row as they lie in memory.  EVEN: F is a multiple of the vector, so a vector lies in the row or behind it.  TAIL: the
+// row's last vector sticks out; where it does, the row's last N elements are loaded instead and moved down when they are used.  NARROW: the
+// row is shorter than a vector: element by element (whose code, next to the others', made every load wait: [32k, 1021] bfloat16 backward
+// 152 us, 76 so).
+enum { EVEN = 0, TAIL = 1, NARROW = 2 };
+typedef unsigned Quad __attribute__((ext_vector_type(4)));
+// q without its first n elements of B bytes (0 <= n < 16 / B), zeros behind
+template <int B> __device__ __forceinline__ Quad quad_drop(Quad q, int n) {
+    const int bytes = n * B;
+    if (bytes & 8) q = Quad{q.z, q.w, 0u, 0u};
+    if (bytes & 4) q = Quad{q.y, q.z, q.w, 0u};
+    if (B == 2 && (bytes & 2))
+        q = Quad{__builtin_amdgcn_alignbit(q.y, q.x, 16), __builtin_amdgcn_alignbit(q.z, q.y, 16), __builtin_amdgcn_alignbit(q.w, q.z, 16), q.w >> 16};
+    return q;
+}
+// the vector at `at` from what raw_fetch loaded: the part behind the row gone
+template <class T, int N, int FIT> __device__ __forceinline__ typename Unaligned<T, N>::type raw_use(typename Unaligned<T, N>::type q, int at, int F) {
+    if constexpr (FIT == TAIL)
+        if (at < F && at + N > F)
+            q = __builtin_bit_cast(typename Unaligned<T, N>::type, quad_drop<(int)sizeof(T)>(__builtin_bit_cast(Quad, q), at + N - F));
+    return q;
+}
+// A load that may stay in flight: q keeps what it held where there is nothing to load (to drop a value is to wait for it: the backward pass of
+// [n, 2944] rows took 150 us instead of 100).  NT: past the caches (a stream that is longer than they are and not read again).
+template <class T, int N, int FIT, bool NT> __device__ __forceinline__ void raw_fetch(typename Unaligned<T, N>::type& q, const T* row, int at, int F, bool on) {
+    typedef typename Unaligned<T, N>::type V;
+    if constexpr (FIT != NARROW) {
+        if (on && at < F) {
+            const V* p = reinterpret_cast<const V*>(row + (FIT == EVEN ? at : min(at, F - N)));
+            if constexpr (NT) q = __builtin_nontemporal_load(p);
+            else q = *p;
+        }
+    } else if (on) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (at + i < F) q[i] = row[at + i];
+    }
+}
+// the vector at `at`, zeros behind the row and for rows that are off: the address is drawn back into the row and the value dropped, without a branch
+template <class T, int N, int FIT, bool NT = false> __device__ __forceinline__ typename Unaligned<T, N>::type raw_load(const T* row, int at, int F, bool on) {
     typedef typename Unaligned<T, N>::type V;
     V q = {};
-    if constexpr (EVEN) {
+    if constexpr (FIT != NARROW) {
         const V* p = reinterpret_cast<const V*>(row + min(at, F - N));
         if constexpr (NT) q = __builtin_nontemporal_load(p);
         else q = *p;
         if (!on || at >= F) q = V{};
-    } else if (on) {
-        if (at + N <= F) {
-            const V* p = reinterpret_cast<const V*>(row + at);
-            if constexpr (NT) q = __builtin_nontemporal_load(p);
-            else q = *p;
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if (at + i < F) q[i] = row[at + i];
-        }
-    }
-    return q;
-}
-// The same for a load that is to stay in flight: q keeps what it held where there is nothing to load (dropping a value means waiting for it:
-// the backward pass of [n, 2944] rows took 150 us instead of 100)
-template <class T, int N, bool EVEN, bool NT> __device__ __forceinline__ void raw_fetch(typename Unaligned<T, N>::type& q, const T* row, int at, int F, bool on) {
-    typedef typename Unaligned<T, N>::type V;
-    if constexpr (EVEN) {
-        if (on && at < F) {
-            if constexpr (NT) q = __builtin_nontemporal_load(reinterpret_cast<const V*>(row + at));
-            else q = *reinterpret_cast<const V*>(row + at);
-        }
-    } else q = raw_load<T, N, false, NT>(row, at, F, on);
+    } else raw_fetch<T, N, FIT, NT>(q, row, at, F, on);
+    return raw_use<T, N, FIT>(q, at, F);
 }
 template <class T, int N> __device__ __forceinline__ void raw_float(const typename Unaligned<T, N>::type& q, float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = (float)q[i];
 }
-template <class T, int N, bool EVEN, bool NT = false> __device__ __forceinline__ void row_load(const T* row, int at, int F, bool on, float (&v)[N]) {
-    raw_float<T, N>(raw_load<T, N, EVEN, NT>(row, at, F, on), v);
+template <class T, int N, int FIT, bool NT = false> __device__ __forceinline__ void row_load(const T* row, int at, int F, bool on, float (&v)[N]) {
+    raw_float<T, N>(raw_load<T, N, FIT, NT>(row, at, F, on), v);
 }
 // v = x + res (res may be NULL)
-template <class T, int N, bool EVEN, bool NT = false> __device__ __forceinline__ void sum_load(const T* x, const T* res, int at, int F, bool on, float (&v)[N]) {
-    row_load<T, N, EVEN, NT>(x, at, F, on, v);
+template <class T, int N, int FIT, bool NT = false> __device__ __forceinline__ void sum_load(const T* x, const T* res, int at, int F, bool on, float (&v)[N]) {
+    row_load<T, N, FIT, NT>(x, at, F, on, v);
     if (res) {
         float r[N];
-        row_load<T, N, EVEN, NT>(res, at, F, on, r);
+        row_load<T, N, FIT, NT>(res, at, F, on, r);
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] += r[i];
     }
 }
 // row[at + i] = v[i], rounded to nearest even, within the row (at < F)
-template <class T, int N, bool EVEN, bool NT = false> __device__ __forceinline__ void row_store(T* row, int at, int F, const float (&v)[N]) {
+template <class T, int N, int FIT, bool NT = false> __device__ __forceinline__ void row_store(T* row, int at, int F, const float (&v)[N]) {
     typedef typename Unaligned<T, N>::type V;
-    if (EVEN || at + N <= F) {
-        V q;
+    V q;
 #pragma unroll
-        for (int i = 0; i < N; i++) q[i] = (T)v[i];
+    for (int i = 0; i < N; i++) q[i] = (T)v[i];
+    if (FIT == EVEN || at + N <= F) {
         if constexpr (NT) __builtin_nontemporal_store(q, reinterpret_cast<V*>(row + at));
         else *reinterpret_cast<V*>(row + at) = q;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            if (at + i < F) row[at + i] = (T)v[i];
+    } else {                        // the bits of the number of bytes that are left
+        Quad w = __builtin_bit_cast(Quad, q);
+        unsigned char* p = reinterpret_cast<unsigned char*>(row + at);
+        const int bytes = (F - at) * (int)sizeof(T);
+        if (bytes & 8) { __builtin_memcpy(p, &w, 8); p += 8; w = Quad{w.z, w.w, 0u, 0u}; }
+        if (bytes & 4) { __builtin_memcpy(p, &w, 4); p += 4; w = Quad{w.y, w.z, w.w, 0u}; }
+        if (sizeof(T) == 2 && (bytes & 2)) { const unsigned short h = (unsigned short)w.x; __builtin_memcpy(p, &h, 2); }
     }
 }
 // the gain: 32 bits or the rows' type; NULL = 1
-template <class T, int N, bool EVEN> __device__ __forceinline__ void gain_load(const void* w, int w32, int at, int F, float (&v)[N]) {
+template <class T, int N, int FIT> __device__ __forceinline__ void gain_load(const void* w, int w32, int at, int F, float (&v)[N]) {
     if (w == nullptr) {
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = 1.0f;
-    } else if (w32) row_load<float, N, EVEN>((const float*)w, at, F, true, v);
-    else row_load<T, N, EVEN>((const T*)w, at, F, true, v);
+    } else if (w32) {
+#pragma unroll
+        for (int h = 0; h < N; h += 4) {
+            float u[4];
+            row_load<float, 4, FIT>((const float*)w, at + h, F, true, u);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[h + i] = u[i];
+        }
+    } else row_load<T, N, FIT>((const T*)w, at, F, true, v);
 }
 
 // ---- sums and maxima over the tpr threads of a row.  Within 16 lanes by DPP (quad_perm, then the mirrors of 8 and 16 lanes: every lane of
@@ -274,17 +299,20 @@ template <int CODE> __device__ __forceinline__ unsigned encode4(const float* t, 
     }
     return in;
 }
-template <int N, bool EVEN> __device__ __forceinline__ void code_store(unsigned char* row, int at, int F, const unsigned (&c)[N / 4]) {
+template <int N, int FIT> __device__ __forceinline__ void code_store(unsigned char* row, int at, int F, const unsigned (&c)[N / 4]) {
     typedef unsigned V __attribute__((ext_vector_type(N / 4), aligned(1)));
-    if (EVEN || at + N <= F) {
+    if (FIT == EVEN || at + N <= F) {
         V q;
 #pragma unroll
         for (int i = 0; i < N / 4; i++) q[i] = c[i];
         *reinterpret_cast<V*>(row + at) = q;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            if (at + i < F) row[at + i] = (unsigned char)(c[i / 4] >> (8 * (i & 3)));
+    } else {                        // the bits of the number of bytes that are left
+        unsigned char* p = row + at;
+        const int bytes = F - at;
+        unsigned w = c[0];
+        if (N == 8 && (bytes & 4)) { __builtin_memcpy(p, &w, 4); p += 4; w = c[N / 4 - 1]; }
+        if (bytes & 2) { const unsigned short h = (unsigned short)w; __builtin_memcpy(p, &h, 2); p += 2; w >>= 16; }
+        if (bytes & 1) *p = (unsigned char)w;
     }
 }
 template <int N> __device__ __forceinline__ unsigned top_bits_of(const float (&v)[N]) {
@@ -354,7 +382,7 @@ struct RmsArgs {
     RowTarget to;
 };
 // NT: the rows are read past the caches.
-template <class T, int NV, int OUT, bool EVEN, bool NT> __global__ __launch_bounds__(512) void rms_forward_kernel(RmsArgs a) {
+template <class T, int NV, int OUT, int FIT, bool NT> __global__ __launch_bounds__(512) void rms_forward_kernel(RmsArgs a) {
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x & a.mask;
@@ -364,7 +392,7 @@ template <class T, int NV, int OUT, bool EVEN, bool NT> __global__ __launch_boun
     const T* res = a.res ? (const T*)a.res + (on ? i : 0) * a.ldr : nullptr;
     float v[NV][N];
 #pragma unroll
-    for (int k = 0; k < NV; k++) sum_load<T, N, EVEN, NT>(x, res, (t + k * tpr) * N, a.F, on, v[k]);
+    for (int k = 0; k < NV; k++) sum_load<T, N, FIT, NT>(x, res, (t + k * tpr) * N, a.F, on, v[k]);
     float rstd = 1.0f;
     if (a.norm) {
         double wide;
@@ -376,12 +404,12 @@ template <class T, int NV, int OUT, bool EVEN, bool NT> __global__ __launch_boun
     for (int k = 0; k < NV; k++) {
         const int at = (t + k * tpr) * N;
         if (at >= a.F || !on) continue;
-        if (a.s) row_store<T, N, EVEN>((T*)a.s + i * a.F, at, a.F, v[k]);
+        if (a.s) row_store<T, N, FIT>((T*)a.s + i * a.F, at, a.F, v[k]);
         float w[N];
-        gain_load<T, N, EVEN>(a.w, a.w32, at, a.F, w);
+        gain_load<T, N, FIT>(a.w, a.w32, at, a.F, w);
 #pragma unroll
         for (int e = 0; e < N; e++) v[k][e] = OUT == 0 ? v[k][e] * rstd * w[e] : v[k][e] * w[e];
-        if constexpr (OUT == 0) row_store<T, N, EVEN>((T*)a.y + i * a.F, at, a.F, v[k]);
+        if constexpr (OUT == 0) row_store<T, N, FIT>((T*)a.y + i * a.F, at, a.F, v[k]);
     }
     if constexpr (OUT != 0) {
         const long long row = row_target(a.to, i, a.rows, t, tpr, lds);
@@ -401,7 +429,7 @@ template <class T, int NV, int OUT, bool EVEN, bool NT> __global__ __launch_boun
             unsigned c[N / 4];
 #pragma unroll
             for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[k][4 * q], g);
-            code_store<N, EVEN>(a.codes + row * a.F, at, a.F, c);
+            code_store<N, FIT>(a.codes + row * a.F, at, a.F, c);
             if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
         }
     }
@@ -421,11 +449,11 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
     unsigned row_top = 0;
     for (int at = t * N; at < a.F; at += tpr * N) {
         float v[N], w[N];
-        sum_load<T, N, false>(x, res, at, a.F, true, v);
+        sum_load<T, N, TAIL>(x, res, at, a.F, true, v);
 #pragma unroll
         for (int e = 0; e < N; e++) ss += (double)v[e] * (double)v[e];
         if (by_row) {
-            gain_load<T, N, false>(a.w, a.w32, at, a.F, w);
+            gain_load<T, N, TAIL>(a.w, a.w32, at, a.F, w);
 #pragma unroll
             for (int e = 0; e < N; e++) v[e] *= w[e];
             row_top = max(row_top, top_bits_of(v));
@@ -441,22 +469,22 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
         const int at = base + t * N;
         const bool in = at < a.F;
         float v[N], w[N];
-        sum_load<T, N, false>(x, res, at, a.F, in, v);
-        if (a.s && in) row_store<T, N, false>((T*)a.s + i * a.F, at, a.F, v);
+        sum_load<T, N, TAIL>(x, res, at, a.F, in, v);
+        if (a.s && in) row_store<T, N, TAIL>((T*)a.s + i * a.F, at, a.F, v);
 #pragma unroll
         for (int e = 0; e < N; e++) w[e] = 0.0f;
-        if (in) gain_load<T, N, false>(a.w, a.w32, at, a.F, w);
+        if (in) gain_load<T, N, TAIL>(a.w, a.w32, at, a.F, w);
 #pragma unroll
         for (int e = 0; e < N; e++) v[e] = OUT == 0 ? v[e] * rstd * w[e] : v[e] * w[e];
         if constexpr (OUT == 0) {
-            if (in) row_store<T, N, false>((T*)a.y + i * a.F, at, a.F, v);
+            if (in) row_store<T, N, TAIL>((T*)a.y + i * a.F, at, a.F, v);
         } else {
             const Group8 g = group_scale<OUT>(seg != 0 ? lanes_max(top_bits_of(v), seg) : row_top);
             if (row >= 0 && in) {
                 unsigned c[N / 4];
 #pragma unroll
                 for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[4 * q], g);
-                code_store<N, false>(a.codes + row * a.F, at, a.F, c);
+                code_store<N, TAIL>(a.codes + row * a.F, at, a.F, c);
                 if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
             }
         }
@@ -481,7 +509,10 @@ struct RmsBackArgs {
     void* ds;               // or NULL: [rows, F]
     float* dw_part;         // or NULL: [gridDim.x, F]
 };
-template <class T, int NV, bool EVEN, bool NT> __global__ __launch_bounds__(512) void rms_backward_kernel(RmsBackArgs a) {
+// Up to 512 threads the next row's loads are in flight while a row is reduced and written; 1024 threads (the widest rows) have no registers for
+// that, but as many waves to hide behind.
+template <class T, int NV, int FIT, bool NT, int MOST> __global__ __launch_bounds__(MOST) void rms_backward_kernel(RmsBackArgs a) {
+    constexpr bool AHEAD = MOST <= 512;
     constexpr int N = RowVec<T>::N;
     typedef typename Unaligned<T, N>::type V;
     __shared__ double lds[2][16];
@@ -493,7 +524,7 @@ template <class T, int NV, bool EVEN, bool NT> __global__ __launch_bounds__(512)
         const int at = (t + k * tpr) * N;
 #pragma unroll
         for (int e = 0; e < N; e++) { dw[k][e] = 0.0f; w[k][e] = 0.0f; }
-        if (at < a.F) gain_load<T, N, EVEN>(a.w, a.w32, at, a.F, w[k]);
+        if (at < a.F) gain_load<T, N, FIT>(a.w, a.w32, at, a.F, w[k]);
     }
     const long long step = (long long)gridDim.x * rpb;
     long long i = (long long)blockIdx.x * rpb + (threadIdx.x >> a.tsh);
@@ -506,32 +537,34 @@ template <class T, int NV, bool EVEN, bool NT> __global__ __launch_bounds__(512)
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int at = (t + k * tpr) * N;
-            raw_fetch<T, N, EVEN, NT>(xq[k], (const T*)a.x + r * a.ldx, at, a.F, on);
-            raw_fetch<T, N, EVEN, NT>(gq[k], (const T*)a.gy + r * a.ldg, at, a.F, on);
-            if (a.res) raw_fetch<T, N, EVEN, NT>(rq[k], (const T*)a.res + r * a.ldr, at, a.F, on);
-            if (a.gs) raw_fetch<T, N, EVEN, NT>(sq[k], (const T*)a.gs + r * a.ldgs, at, a.F, on);
+            raw_fetch<T, N, FIT, NT>(xq[k], (const T*)a.x + r * a.ldx, at, a.F, on);
+            raw_fetch<T, N, FIT, NT>(gq[k], (const T*)a.gy + r * a.ldg, at, a.F, on);
+            if (a.res) raw_fetch<T, N, FIT, NT>(rq[k], (const T*)a.res + r * a.ldr, at, a.F, on);
+            if (a.gs) raw_fetch<T, N, FIT, NT>(sq[k], (const T*)a.gs + r * a.ldgs, at, a.F, on);
         }
     };
-    fetch(i);
+    if (AHEAD) fetch(i);
     int turn = 0;
     for (long long r0 = (long long)blockIdx.x * rpb; r0 < a.rows; r0 += step, i += step, turn ^= 1) {
         const bool on = i < a.rows;
+        if (!AHEAD) fetch(i);
         const float rs = rstd;
         float h[NV][N], g[NV][N], c[N];
         V q[NV];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
-            raw_float<T, N>(xq[k], h[k]);
-            raw_float<T, N>(gq[k], g[k]);
-            if (a.gs) q[k] = sq[k];
+            const int at = (t + k * tpr) * N;
+            raw_float<T, N>(raw_use<T, N, FIT>(xq[k], at, a.F), h[k]);
+            raw_float<T, N>(raw_use<T, N, FIT>(gq[k], at, a.F), g[k]);
+            if (a.gs) q[k] = raw_use<T, N, FIT>(sq[k], at, a.F);
             if (a.res) {
                 float r[N];
-                raw_float<T, N>(rq[k], r);
+                raw_float<T, N>(raw_use<T, N, FIT>(rq[k], at, a.F), r);
 #pragma unroll
                 for (int e = 0; e < N; e++) h[k][e] += r[e];
             }
         }
-        fetch(i + step);                        // in flight while this row is reduced and written
+        if (AHEAD) fetch(i + step);             // in flight while this row is reduced and written
 #pragma unroll
         for (int e = 0; e < N; e++) c[e] = 0.0f;
         // (a vector behind the row holds zeros; a row that is off holds an earlier one and has no part in dw)
@@ -564,7 +597,7 @@ template <class T, int NV, bool EVEN, bool NT> __global__ __launch_bounds__(512)
 #pragma unroll
                 for (int e = 0; e < N; e++) d[e] += u[e];
             }
-            row_store<T, N, EVEN, NT>((T*)a.ds + i * a.F, at, a.F, d);
+            row_store<T, N, FIT, NT>((T*)a.ds + i * a.F, at, a.F, d);
         }
     }
     if (a.dw_part == nullptr) return;
@@ -583,12 +616,18 @@ template <class T, int NV, bool EVEN, bool NT> __global__ __launch_bounds__(512)
 #pragma unroll
                 for (int e = 0; e < N; e++) part[wave][lane * N + e] = dw[k][e];
             __syncthreads();
-            if (threadIdx.x < tpr)
+            if ((int)threadIdx.x < tpr)
                 for (int q = 1; q < (int)(blockDim.x >> 6); q++)
 #pragma unroll
                     for (int e = 0; e < N; e++) dw[k][e] += part[q][lane * N + e];
         }
-        if (threadIdx.x < tpr && at < a.F) row_store<float, N, EVEN>(out, at, a.F, dw[k]);
+        if ((int)threadIdx.x < tpr)
+#pragma unroll
+            for (int h = 0; h < N; h += 4)
+                if (at + h < a.F) {
+                    const float d[4] = {dw[k][h], dw[k][h + 1], dw[k][h + 2], dw[k][h + 3]};
+                    row_store<float, 4, FIT>(out, at + h, a.F, d);
+                }
     }
 }
 // rows beyond the registers: ds by one workgroup per row (read twice), dw by columns
@@ -604,9 +643,9 @@ template <class T> __global__ __launch_bounds__(512) void rms_backward_long_kern
     double c = 0.0;
     for (int at = t * N; at < a.F; at += tpr * N) {
         float h[N], g[N], w[N];
-        sum_load<T, N, false>(x, res, at, a.F, true, h);
-        row_load<T, N, false>(gy, at, a.F, true, g);
-        gain_load<T, N, false>(a.w, a.w32, at, a.F, w);
+        sum_load<T, N, TAIL>(x, res, at, a.F, true, h);
+        row_load<T, N, TAIL>(gy, at, a.F, true, g);
+        gain_load<T, N, TAIL>(a.w, a.w32, at, a.F, w);
         float p = 0.0f;
 #pragma unroll
         for (int e = 0; e < N; e++) p += g[e] * w[e] * (h[e] * rstd);
@@ -615,30 +654,41 @@ template <class T> __global__ __launch_bounds__(512) void rms_backward_long_kern
     const float mean = (float)row_sum(c, tpr, lds, 0) / (float)a.F;
     for (int at = t * N; at < a.F; at += tpr * N) {
         float h[N], g[N], w[N], d[N];
-        sum_load<T, N, false>(x, res, at, a.F, true, h);
-        row_load<T, N, false>(gy, at, a.F, true, g);
-        gain_load<T, N, false>(a.w, a.w32, at, a.F, w);
+        sum_load<T, N, TAIL>(x, res, at, a.F, true, h);
+        row_load<T, N, TAIL>(gy, at, a.F, true, g);
+        gain_load<T, N, TAIL>(a.w, a.w32, at, a.F, w);
 #pragma unroll
         for (int e = 0; e < N; e++) d[e] = rstd * (g[e] * w[e] - h[e] * rstd * mean);
         if (a.gs) {
             float q[N];
-            row_load<T, N, false>((const T*)a.gs + i * a.ldgs, at, a.F, true, q);
+            row_load<T, N, TAIL>((const T*)a.gs + i * a.ldgs, at, a.F, true, q);
 #pragma unroll
             for (int e = 0; e < N; e++) d[e] += q[e];
         }
-        row_store<T, N, false>((T*)a.ds + i * a.F, at, a.F, d);
+        row_store<T, N, TAIL>((T*)a.ds + i * a.F, at, a.F, d);
     }
 }
 template <class T> __global__ __launch_bounds__(256) void rms_dw_columns_kernel(RmsBackArgs a, int slices) {
-    const long long col = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (col >= a.F) return;
-    float sum = 0.0f;
+    constexpr int N = RowVec<T>::N;
+    const int at = ((int)blockIdx.x * 256 + (int)threadIdx.x) * N;
+    if (at >= a.F) return;
+    float sum[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) sum[e] = 0.0f;
     for (long long i = blockIdx.y; i < a.rows; i += slices) {
-        float v = (float)((const T*)a.x)[i * a.ldx + col];
-        if (a.res) v += (float)((const T*)a.res)[i * a.ldr + col];
-        sum += (float)((const T*)a.gy)[i * a.ldg + col] * (v * a.rstd[i]);
+        const float rstd = a.rstd[i];
+        float h[N], g[N];
+        sum_load<T, N, TAIL>((const T*)a.x + i * a.ldx, a.res ? (const T*)a.res + i * a.ldr : nullptr, at, a.F, true, h);
+        row_load<T, N, TAIL>((const T*)a.gy + i * a.ldg, at, a.F, true, g);
+#pragma unroll
+        for (int e = 0; e < N; e++) sum[e] += g[e] * (h[e] * rstd);
     }
-    a.dw_part[(long long)blockIdx.y * a.F + col] = sum;
+#pragma unroll
+    for (int h = 0; h < N; h += 4)
+        if (at + h < a.F) {
+            const float d[4] = {sum[h], sum[h + 1], sum[h + 2], sum[h + 3]};
+            row_store<float, 4, TAIL>(a.dw_part + (long long)blockIdx.y * a.F, at + h, a.F, d);
+        }
 }
 // dw = the sum of n partial rows, in a fixed order: 32 columns and 32 slices of the partials per workgroup, eight loads in flight each (a
 // narrow table has one workgroup here and up to 2048 partials: what counts is the number of loads that wait for each other)
@@ -676,29 +726,35 @@ struct ReadArgs {
     void* out;              // [rows, F]
 };
 // the codes of N columns and their scale as values, zeros beyond the row and for rows that are off
-template <int CODE, int N, bool EVEN> __device__ __forceinline__ void code_load(const ReadArgs& a, long long row, int at, float (&v)[N]) {
+template <int CODE, int N, int FIT> __device__ __forceinline__ void code_load(const ReadArgs& a, long long row, int at, float (&v)[N]) {
     const unsigned char* codes = a.codes + (row >= 0 ? row : 0) * a.F;
     const bool in = row >= 0 && at < a.F;
-    const int p = EVEN ? min(at, a.F - N) : at;
+    const int p = FIT != NARROW ? min(at, a.F - N) : at;
     float scale = 0.0f;
     unsigned c[N / 4] = {};
     if (a.P > 0) {          // (an empty table has nothing to draw the address back to)
-        if (EVEN || in) scale = a.scales[(row >= 0 ? row : 0) * a.groups + (p >> a.gshift)];
-        if (EVEN || (in && at + N <= a.F)) __builtin_memcpy(c, codes + p, N);
+        scale = a.scales[(row >= 0 ? row : 0) * a.groups + (min(at, a.F - 1) >> a.gshift)];
+        if (FIT != NARROW) __builtin_memcpy(c, codes + p, N);
         else if (in)
             for (int e = 0; e < N && at + e < a.F; e++) c[e / 4] |= (unsigned)codes[at + e] << (8 * (e & 3));
+        if (FIT == TAIL && in && at > p) {        // the row's last N codes: those in front of `at` go
+            unsigned long long w = 0;
+            __builtin_memcpy(&w, c, N);
+            w >>= 8 * (at - p);
+            __builtin_memcpy(c, &w, N);
+        }
     }
 #pragma unroll
     for (int q = 0; q < N / 4; q++) Code8<CODE>::unpack4(c[q], v + 4 * q);
 #pragma unroll
-    for (int e = 0; e < N; e++) v[e] = in && (EVEN || at + e < a.F) ? v[e] * scale : 0.0f;
+    for (int e = 0; e < N; e++) v[e] = in && (FIT == EVEN || at + e < a.F) ? v[e] * scale : 0.0f;
 }
 __device__ __forceinline__ long long read_row(const ReadArgs& a, long long i) {
     const long long row = a.index == nullptr ? a.first + i : a.is64 ? ((const long long*)a.index)[i] : (long long)((const int*)a.index)[i];
     return row < a.P ? row : -1;
 }
 // NT: written past the caches.
-template <class T, int CODE, int NV, bool EVEN, bool NT> __global__ __launch_bounds__(512) void rows_read_kernel(ReadArgs a) {
+template <class T, int CODE, int NV, int FIT, bool NT> __global__ __launch_bounds__(512) void rows_read_kernel(ReadArgs a) {
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x & a.mask;
@@ -706,7 +762,7 @@ template <class T, int CODE, int NV, bool EVEN, bool NT> __global__ __launch_bou
     const long long row = i < a.rows ? read_row(a, i) : -1;
     float v[NV][N];
 #pragma unroll
-    for (int k = 0; k < NV; k++) code_load<CODE, N, EVEN>(a, row, (t + k * tpr) * N, v[k]);
+    for (int k = 0; k < NV; k++) code_load<CODE, N, FIT>(a, row, (t + k * tpr) * N, v[k]);
     float inv = 1.0f;
     if (a.norm) {
         double wide;
@@ -719,7 +775,7 @@ template <class T, int CODE, int NV, bool EVEN, bool NT> __global__ __launch_bou
         const int at = (t + k * tpr) * N;
 #pragma unroll
         for (int e = 0; e < N; e++) v[k][e] *= inv;
-        if (at < a.F) row_store<T, N, EVEN, NT>((T*)a.out + i * a.F, at, a.F, v[k]);
+        if (at < a.F) row_store<T, N, FIT, NT>((T*)a.out + i * a.F, at, a.F, v[k]);
     }
 }
 template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_long_kernel(ReadArgs a) {
@@ -732,7 +788,7 @@ template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_lo
         double ss = 0.0;
         for (int at = t * N; at < a.F; at += tpr * N) {
             float v[N];
-            code_load<CODE, N, false>(a, row, at, v);
+            code_load<CODE, N, TAIL>(a, row, at, v);
 #pragma unroll
             for (int e = 0; e < N; e++) ss += (double)v[e] * (double)v[e];
         }
@@ -741,10 +797,10 @@ template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_lo
     }
     for (int at = t * N; at < a.F; at += tpr * N) {
         float v[N];
-        code_load<CODE, N, false>(a, row, at, v);
+        code_load<CODE, N, TAIL>(a, row, at, v);
 #pragma unroll
         for (int e = 0; e < N; e++) v[e] *= inv;
-        row_store<T, N, false>((T*)a.out + i * a.F, at, a.F, v);
+        row_store<T, N, TAIL>((T*)a.out + i * a.F, at, a.F, v);
     }
 }
 

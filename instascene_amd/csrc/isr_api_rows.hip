@@ -34,7 +34,7 @@ constexpr long long NT_BACKWARD = 64ll << 20, NT_CODES = 128ll << 20;
 // and backward, 333 with 4, 456 with 8), as many waves as the row needs.  Where there are so few rows that the chip would stand idle, 1 vector
 // per thread.
 struct RowShape { int tpr, mask, tsh, rpb, nv, block; };
-RowShape row_shape(int vecs, long long rows, int least, int max_nv) {
+RowShape row_shape(int vecs, long long rows, int least, int max_nv, int max_waves = 8) {
     int tsh = 0;
     while ((1 << tsh) < vecs && tsh < 6) tsh++;
     while (tsh > 0 && (vecs + (1 << (tsh - 1)) - 1) >> (tsh - 1) <= least && (rows << (tsh - 1)) >= 2048 * 256) tsh--;
@@ -42,16 +42,17 @@ RowShape row_shape(int vecs, long long rows, int least, int max_nv) {
     if (per_lane <= (tsh == 6 && rows * 64 < 256 * 256 ? 1 : 2)) return {1 << tsh, (1 << tsh) - 1, tsh, 256 >> tsh, per_lane, 256};
     for (int nv = rows * ((vecs + 1) / 2) < 256 * 256 ? 1 : 2; nv <= max_nv; nv *= 2) {
         const int waves = (vecs + 64 * nv - 1) / (64 * nv);
-        if (waves <= 8) return {64 * waves, 0x7fffffff, 31, 1, nv, 64 * waves};
+        if (waves <= max_waves) return {64 * waves, 0x7fffffff, 31, 1, nv, 64 * waves};
     }
     return {512, 0x7fffffff, 31, 1, 0, 512};
 }
 template <class A> void set_shape(A& a, const RowShape& r) { a.tpr = r.tpr; a.mask = r.mask; a.tsh = r.tsh; a.rpb = r.rpb; }
 
-#define ROWS_NV(nv, even, call, call_long) \
-    do { if (nv == 1) { if (even) { call(1, true); } else { call(1, false); } } else if (nv == 2) { if (even) { call(2, true); } else { call(2, false); } } \
-         else if (nv == 4) { if (even) { call(4, true); } else { call(4, false); } } else if (nv == 8) { if (even) { call(8, true); } else { call(8, false); } } \
-         else { call_long; } } while (0)
+#define ROWS_NV(nv, fit, call, call_long) \
+    do { if (fit == iso::NARROW) { call(1, iso::NARROW); } else if (nv == 0) { call_long; } \
+         else if (fit == iso::EVEN) { if (nv == 1) { call(1, iso::EVEN); } else if (nv == 2) { call(2, iso::EVEN); } else if (nv == 4) { call(4, iso::EVEN); } else { call(8, iso::EVEN); } } \
+         else { if (nv == 1) { call(1, iso::TAIL); } else if (nv == 2) { call(2, iso::TAIL); } else if (nv == 4) { call(4, iso::TAIL); } else { call(8, iso::TAIL); } } } while (0)
+template <class T> int row_fit(int F) { return F < iso::RowVec<T>::N ? iso::NARROW : F % iso::RowVec<T>::N ? iso::TAIL : iso::EVEN; }
 
 template <class T, int OUT> void launch_forward(iso::RmsArgs a, hipStream_t s) {
     constexpr int N = iso::RowVec<T>::N;
@@ -59,16 +60,17 @@ template <class T, int OUT> void launch_forward(iso::RmsArgs a, hipStream_t s) {
     set_shape(a, sh);
     const int nv = sh.nv;
     // (past the caches only whole 128-byte lines per load: [8 M, 32] float32 224 us so with 4 threads per row, 174 cached)
-    const bool nt = OUT != 0 && a.tpr >= 8 && a.rows * a.F * (long long)sizeof(T) >= NT_CODES, even = a.F % N == 0;
+    const bool nt = OUT != 0 && a.tpr >= 8 && a.rows * a.F * (long long)sizeof(T) >= NT_CODES;
+    const int fit = row_fit<T>(a.F);
     const int block = sh.block, rpb = sh.rpb;
     const long long step = MAX_THREADS / block * rpb;
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
         const dim3 grid((unsigned)((n + rpb - 1) / rpb));
-#define FWD(NV, EVEN) do { if (OUT != 0 && nt) hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, EVEN, OUT != 0>), grid, dim3(block), 0, s, a); \
-                           else hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, EVEN, false>), grid, dim3(block), 0, s, a); } while (0)
+#define FWD(NV, FIT) do { if (OUT != 0 && nt) hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, FIT, OUT != 0>), grid, dim3(block), 0, s, a); \
+                           else hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, FIT, false>), grid, dim3(block), 0, s, a); } while (0)
 #define FWD_LONG hipLaunchKernelGGL((iso::rms_forward_long_kernel<T, OUT>), grid, dim3(block), 0, s, a)
-        ROWS_NV(nv, even, FWD, FWD_LONG);
+        ROWS_NV(nv, fit, FWD, FWD_LONG);
 #undef FWD
 #undef FWD_LONG
     }
@@ -86,8 +88,12 @@ void launch_codes(int code, int type, const iso::RmsArgs& a, hipStream_t s) {
 // workgroups of the backward pass = partial rows of dw: enough to keep the memory busy (two of 256 threads per compute unit do for wide rows:
 // 768 and 1024 workgroups took 1 to 14 % longer at [n, 2048..4096] float32), few enough that the partials stay small against the rows
 template <class T> RowShape backward_shape(long long rows, int F, int& grid) {
-    const RowShape sh = row_shape((F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, rows, 1, 4);
-    if (sh.nv == 0) { grid = (int)std::min<long long>(64, std::max<long long>(1, rows)); return sh; }       // slices of the columns' sums
+    const RowShape sh = row_shape((F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, rows, 1, 2, sizeof(T) == 4 ? 16 : 8);       // (what the registers hold)
+    if (sh.nv == 0) {           // slices of the columns' sums: 1024 workgroups with those that the columns need
+        const int cols = 256 * iso::RowVec<T>::N;
+        grid = (int)std::max<long long>(1, std::min<long long>(rows, std::max(16, 1024 / ((F + cols - 1) / cols))));
+        return sh;
+    }
     const long long need = (rows + sh.rpb - 1) / sh.rpb, most = std::max<long long>(512, std::min<long long>(2048, (1 << 20) / F));
     grid = (int)std::max<long long>(1, std::min(need, most));
     return sh;
@@ -95,40 +101,43 @@ template <class T> RowShape backward_shape(long long rows, int F, int& grid) {
 RowShape backward_shape_type(int type, long long rows, int F, int& grid) {
     return type == 0 ? backward_shape<float>(rows, F, grid) : type == 1 ? backward_shape<__bf16>(rows, F, grid) : backward_shape<_Float16>(rows, F, grid);
 }
-template <class T, bool EVEN, bool NT> void launch_backward_nv(const iso::RmsBackArgs& a, int nv, int block, int grid, hipStream_t s) {
-    if (nv == 1) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 1, EVEN, NT>), dim3(grid), dim3(block), 0, s, a);
-    else if (nv == 2) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 2, EVEN, NT>), dim3(grid), dim3(block), 0, s, a);
-    else hipLaunchKernelGGL((iso::rms_backward_kernel<T, 4, EVEN, NT>), dim3(grid), dim3(block), 0, s, a);
+template <class T, int FIT, bool NT> void launch_backward_fit(const iso::RmsBackArgs& a, int nv, int block, int grid, hipStream_t s) {
+    if (nv == 1) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 1, FIT, NT, 512>), dim3(grid), dim3(block), 0, s, a);
+    else if (block <= 512) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 2, FIT, NT, 512>), dim3(grid), dim3(block), 0, s, a);
+    else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 2, FIT, NT, 1024>), dim3(grid), dim3(block), 0, s, a);
 }
 template <class T> void launch_backward(iso::RmsBackArgs a, int nv, int block, int grid, hipStream_t s) {
     if (nv != 0) {
-        const bool even = a.F % iso::RowVec<T>::N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= NT_BACKWARD;
-        if (even && nt) launch_backward_nv<T, true, true>(a, nv, block, grid, s);
-        else if (even) launch_backward_nv<T, true, false>(a, nv, block, grid, s);
-        else if (nt) launch_backward_nv<T, false, true>(a, nv, block, grid, s);
-        else launch_backward_nv<T, false, false>(a, nv, block, grid, s);
+        const int fit = row_fit<T>(a.F);
+        const bool nt = a.rows * a.F * (long long)sizeof(T) >= NT_BACKWARD;
+        if (fit == iso::NARROW) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 1, iso::NARROW, false, 512>), dim3(grid), dim3(block), 0, s, a);
+        else if (fit == iso::EVEN && nt) launch_backward_fit<T, iso::EVEN, true>(a, nv, block, grid, s);
+        else if (fit == iso::EVEN) launch_backward_fit<T, iso::EVEN, false>(a, nv, block, grid, s);
+        else if (nt) launch_backward_fit<T, iso::TAIL, true>(a, nv, block, grid, s);
+        else launch_backward_fit<T, iso::TAIL, false>(a, nv, block, grid, s);
         return;
     }
     if (a.ds)
         for (a.row0 = 0; a.row0 < a.rows; a.row0 += MAX_THREADS / 512)
             hipLaunchKernelGGL((iso::rms_backward_long_kernel<T>), dim3((unsigned)std::min(MAX_THREADS / 512, a.rows - a.row0)), dim3(512), 0, s, a);
-    if (a.dw_part) hipLaunchKernelGGL((iso::rms_dw_columns_kernel<T>), dim3((a.F + 255) / 256, grid), dim3(256), 0, s, a, grid);
+    if (a.dw_part) hipLaunchKernelGGL((iso::rms_dw_columns_kernel<T>), dim3((a.F + 256 * iso::RowVec<T>::N - 1) / (256 * iso::RowVec<T>::N), grid), dim3(256), 0, s, a, grid);
 }
 template <class T, int CODE> void launch_read(iso::ReadArgs a, hipStream_t s) {
     constexpr int N = iso::RowVec<T>::N;
     const RowShape sh = row_shape((a.F + N - 1) / N, a.rows, 2, 8);
     set_shape(a, sh);
     const int nv = sh.nv;
-    const bool even = a.F % N == 0, nt = a.rows * a.F * (long long)sizeof(T) >= NT_CODES;
+    const int fit = row_fit<T>(a.F);
+    const bool nt = a.rows * a.F * (long long)sizeof(T) >= NT_CODES;
     const int block = sh.block, rpb = sh.rpb;
     const long long step = MAX_THREADS / block * rpb;
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
         const dim3 grid((unsigned)((n + rpb - 1) / rpb));
-#define READ(NV, EVEN) do { if (nt) hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, EVEN, true>), grid, dim3(block), 0, s, a); \
-                            else hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, EVEN, false>), grid, dim3(block), 0, s, a); } while (0)
+#define READ(NV, FIT) do { if (nt) hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, FIT, true>), grid, dim3(block), 0, s, a); \
+                            else hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, FIT, false>), grid, dim3(block), 0, s, a); } while (0)
 #define READ_LONG hipLaunchKernelGGL((iso::rows_read_long_kernel<T, CODE>), grid, dim3(block), 0, s, a)
-        ROWS_NV(nv, even, READ, READ_LONG);
+        ROWS_NV(nv, fit, READ, READ_LONG);
 #undef READ
 #undef READ_LONG
     }
