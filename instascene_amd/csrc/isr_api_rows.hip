@@ -232,7 +232,8 @@ int iso_rows8_write(int type, int code, long long n, int F, int group, long long
     hipStream_t s = (hipStream_t)stream;
     if (!code_type(code)) return fail(ISR_EINVAL, "rows8_write: code %d is neither 1 (int8) nor 2 (e4m3)", code);
     if (!group_ok(F, group)) return fail(ISR_EINVAL, "rows8_write: groups of %d columns do not fit rows of %d", group, F);
-    if (P < 0 || n > 0x7fffffffll || (!index && (first < 0 || first + n > P))) return fail(ISR_EINVAL, "rows8_write: rows [%lld, %lld) of a table of %lld", first, first + n, P);
+    if (index && n > 0x7fffffffll) return fail(ISR_EINVAL, "rows8_write: at most 2^31 - 1 indices in one call");
+    if (P < 0 || (!index && (first < 0 || first > P || n > P - first))) return fail(ISR_EINVAL, "rows8_write: rows [%lld, %lld) of a table of %lld", first, first + n, P);
     if (n == 0 || P == 0) return ISR_OK;
     if (!rows || !codes || !scales) return fail(ISR_EINVAL, "rows8_write: null pointer");
     if (index && n > ISO_ROWS8_SCAN && !owner) return fail(ISR_EINVAL, "rows8_write: more than %d indices need the owner table", ISO_ROWS8_SCAN);
@@ -256,7 +257,7 @@ int iso_rows8_read(int type, int code, long long n, int F, int group, long long 
     hipStream_t s = (hipStream_t)stream;
     if (!code_type(code)) return fail(ISR_EINVAL, "rows8_read: code %d is neither 1 (int8) nor 2 (e4m3)", code);
     if (!group_ok(F, group)) return fail(ISR_EINVAL, "rows8_read: groups of %d columns do not fit rows of %d", group, F);
-    if (P < 0 || (!index && (first < 0 || first + n > P))) return fail(ISR_EINVAL, "rows8_read: rows [%lld, %lld) of a table of %lld", first, first + n, P);
+    if (P < 0 || (!index && (first < 0 || first > P || n > P - first))) return fail(ISR_EINVAL, "rows8_read: rows [%lld, %lld) of a table of %lld", first, first + n, P);
     if (n == 0) return ISR_OK;
     if (!out || (P > 0 && (!codes || !scales))) return fail(ISR_EINVAL, "rows8_read: null pointer");
     iso::ReadArgs a = {};

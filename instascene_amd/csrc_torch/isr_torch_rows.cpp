@@ -119,10 +119,10 @@ public:
             at::AutoGradMode off(false);
             out = gradients(ctx, grads[0], grads.size() > 1 ? grads[1] : Tensor());
         }
-        if (again && std::any_of(grads.begin(), grads.end(), [](const Tensor& g) { return g.defined() && g.requires_grad(); })) {
+        if (again) {                    // an error for whoever does differentiate them
             torch::autograd::variable_list some;
             for (const Tensor& t : out)
-                if (t.defined()) some.push_back(t);
+                if (t.defined()) some.push_back(t.detach().set_requires_grad(true));
             auto error = std::make_shared<torch::autograd::DelayedError>("rms_norm: the gradients of its backward pass are not available", (int)some.size());
             some = (*error)(std::move(some));
             size_t k = 0;

@@ -194,6 +194,8 @@ class SegTrainer:
         self.prefetch_mode = _os.environ.get("ISR_PREFETCH_MODE", "behind" if _pe is None else ("early" if _pe == "1" else "after"))
         self.high_priority_main = _os.environ.get("ISR_MAIN_PRIORITY", "1") == "1"     # measured: 2.03 -> 1.995 ms per C3 step
         self.sharded_tail = _os.environ.get("ISR_SHARDED_TAIL", "0") == "1"    # opt-in (unmeasured on hardware): _tail_sharded
+        if self.max_grad_norm is not None and self.sharded_tail and world > 1:
+            raise ValueError("SegTrainer: max_grad_norm is not supported by the sharded tail (no rank has the whole gradient)")
         # how the multi-rank tail sums dL/dparam: "rccl" (default: torch.distributed all-reduce in row ranges), "peer" (direct
         # reduce-scatter / all-gather over peer-mapped buffers) or "peer_compact" (only the rows this step touched) -
         # peer_exchange.PeerExchange, device-side phase flags; opt-in (ISR_EXCHANGE): never timed on a multi-GPU node

@@ -6,6 +6,7 @@ synchronises nothing, so it can be captured into a graph."""
 from __future__ import annotations
 
 import functools
+import operator
 from typing import Optional
 
 import torch
@@ -17,7 +18,8 @@ CODE_TYPES = (torch.int8, torch.float8_e4m3fn)
 
 @functools.lru_cache(maxsize=None)
 def _ext():
-    """The compiled host side (csrc_torch/isr_torch_rows.cpp): checks, allocation, the autograd node, the launches.  No fallback."""
+    """The compiled host side (csrc_torch/isr_torch_rows.cpp): checks, allocation, the autograd node, the launches.  No fallback.  (It is
+    linked to the library beside it: an A/B build named by ISR_LIB_PATH does not reach these operators.)"""
     from . import _lib
     _lib.lib()              # torch's HIP runtime first, then the library: one runtime in the process
     try:
@@ -110,11 +112,11 @@ class QuantizedRows:
         if index is None:
             if rows.shape[0] != P:
                 raise ValueError(f"{what}: {rows.shape[0]} rows for a table of {P}; give an index")
-        elif isinstance(index, int):
-            first = index
+        elif not isinstance(index, torch.Tensor):
+            first = operator.index(index)
         else:
             ix = index
-            if self._owner is None and ix.shape[0] > SCAN_MAX:
+            if self._owner is None and ix.numel() > SCAN_MAX:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError(f"{what}: the first write of more than {SCAN_MAX} indices to this table makes a helper table and "
                                        "cannot be captured: write once before the capture")
@@ -134,7 +136,7 @@ class QuantizedRows:
                 raise ValueError(f"QuantizedRows.read: a slice of step 1, not {step}")
             n = max(0, stop - first)
             first = first if n else 0
-        else:
+        elif index is not None:
             ix = index
         return _ext().rows8_read(self.codes, self.scales, ix, first, n, out_dtype, norm_eps)
 

@@ -8,11 +8,10 @@ import random
 import pytest
 import torch
 
-pytestmark = pytest.mark.gpu
+from instascene_amd._lib import IsrError
+from instascene_amd.optim import clip_grad_norm_, clip_grads_, grad_norm
 
-if torch.cuda.is_available():
-    from instascene_amd._lib import IsrError
-    from instascene_amd.optim import clip_grad_norm_, clip_grads_, grad_norm
+pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
 TYPES = [torch.float32, torch.bfloat16, torch.float16]

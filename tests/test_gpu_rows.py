@@ -9,11 +9,10 @@ import math
 import pytest
 import torch
 
-pytestmark = pytest.mark.gpu
+from instascene_amd.contrastive import gather_rows, row_normalize
+from instascene_amd.rows import SCAN_MAX, QuantizedRows, rms_norm, rms_norm_quantized
 
-if torch.cuda.is_available():
-    from instascene_amd.contrastive import gather_rows, row_normalize
-    from instascene_amd.rows import SCAN_MAX, QuantizedRows, rms_norm, rms_norm_quantized
+pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -125,6 +124,33 @@ def test_rms_norm_backward_long_sums_and_partial_gradients():
     check(dw, (gy.double() * h).sum(0), (gy.double() * h).abs().sum(0) * 512 * U, "dw")   # <= 30001 / 2048 / 32 + 4 + 2048 / 8 + 8 terms in turn
     y, s = rms_norm(x, w, 1e-6, residual=r)
     assert torch.equal(torch.autograd.grad(s, x, gy)[0], gy)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("width", [3, 100, 4100, 20003])
+def test_rms_norm_gradients_of_one_input_at_a_time(dtype, width):
+    """Each gradient alone has the bits it has beside the others; an expanded incoming gradient; 64 rows per partial sum and more."""
+    x, r, w = make((150, width), dtype, 1), make((150, width), dtype, 2), 1.0 + 0.1 * make((width,), F32, 3)
+    gy = make((150, width), dtype, 4)
+
+    def grads(*wanted):
+        leaves = [t.clone().requires_grad_(k in wanted) for k, t in enumerate((x, r, w))]
+        y, _ = rms_norm(leaves[0], leaves[2], 1e-6, residual=leaves[1])
+        return dict(zip(wanted, torch.autograd.grad(y, [leaves[k] for k in wanted], gy)))
+
+    whole = grads(0, 1, 2)
+    assert torch.equal(whole[0], whole[1])
+    for k in range(3):
+        assert torch.equal(grads(k)[k], whole[k])
+    leaf = x.clone().requires_grad_(True)
+    rms_norm(leaf, w).sum().backward()                      # (a gradient of one element, expanded)
+    again, = torch.autograd.grad(rms_norm(leaf, w), leaf, torch.ones_like(x))
+    assert torch.equal(leaf.grad, again)
+    for incoming in (gy, gy.clone().requires_grad_(True)):
+        g, = torch.autograd.grad(rms_norm(leaf, w), leaf, incoming, create_graph=True)
+        assert torch.equal(g, torch.autograd.grad(rms_norm(leaf, w), leaf, gy)[0])
+        with pytest.raises(RuntimeError, match="backward pass"):
+            g.sum().backward()
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
