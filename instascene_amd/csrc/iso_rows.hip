@@ -510,7 +510,7 @@ struct RmsBackArgs {
     float* dw_part;         // or NULL: [gridDim.x, F]
 };
 // Up to 512 threads the next row's loads are in flight while a row is reduced and written; 1024 threads (the widest rows) have no registers for
-// that, but as many waves to hide behind.
+// that, nor for the gain (read again for every row, from the caches), but as many waves to hide behind.
 template <class T, int NV, int FIT, bool NT, int MOST> __global__ __launch_bounds__(MOST) void rms_backward_kernel(RmsBackArgs a) {
     constexpr bool AHEAD = MOST <= 512;
     constexpr int N = RowVec<T>::N;
@@ -524,7 +524,7 @@ template <class T, int NV, int FIT, bool NT, int MOST> __global__ __launch_bound
         const int at = (t + k * tpr) * N;
 #pragma unroll
         for (int e = 0; e < N; e++) { dw[k][e] = 0.0f; w[k][e] = 0.0f; }
-        if (at < a.F) gain_load<T, N, FIT>(a.w, a.w32, at, a.F, w[k]);
+        if (AHEAD && at < a.F) gain_load<T, N, FIT>(a.w, a.w32, at, a.F, w[k]);
     }
     const long long step = (long long)gridDim.x * rpb;
     long long i = (long long)blockIdx.x * rpb + (threadIdx.x >> a.tsh);
@@ -547,7 +547,71 @@ template <class T, int NV, int FIT, bool NT, int MOST> __global__ __launch_bound
     int turn = 0;
     for (long long r0 = (long long)blockIdx.x * rpb; r0 < a.rows; r0 += step, i += step, turn ^= 1) {
         const bool on = i < a.rows;
-        if (!AHEAD) fetch(i);
+        if constexpr (!AHEAD) {
+            // the raw vectors stay, h and gy w are formed twice
+#pragma unroll
+            for (int k = 0; k < NV; k++) xq[k] = rq[k] = gq[k] = sq[k] = V{};
+            fetch(i);
+            float c[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) c[e] = 0.0f;
+            auto terms = [&](int k, float (&h)[N], float (&g)[N]) {
+                raw_float<T, N>(xq[k], h);
+                raw_float<T, N>(gq[k], g);
+                if (a.res) {
+                    float r[N];
+                    raw_float<T, N>(rq[k], r);
+#pragma unroll
+                    for (int e = 0; e < N; e++) h[e] += r[e];
+                }
+#pragma unroll
+                for (int e = 0; e < N; e++) h[e] *= rstd;
+            };
+            auto times_gain = [&](int at, float (&g)[N]) {
+                float u[N];
+                gain_load<T, N, FIT>(a.w, a.w32, at, a.F, u);
+#pragma unroll
+                for (int e = 0; e < N; e++) g[e] *= u[e];
+            };
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int at = (t + k * tpr) * N;
+                if (at >= a.F) continue;
+                xq[k] = raw_use<T, N, FIT>(xq[k], at, a.F);
+                gq[k] = raw_use<T, N, FIT>(gq[k], at, a.F);
+                rq[k] = raw_use<T, N, FIT>(rq[k], at, a.F);
+                float h[N], g[N];
+                terms(k, h, g);
+#pragma unroll
+                for (int e = 0; e < N; e++) dw[k][e] = __builtin_fmaf(g[e], h[e], dw[k][e]);        // (the workgroup is one row: on)
+                times_gain(at, g);
+#pragma unroll
+                for (int e = 0; e < N; e++) c[e] = __builtin_fmaf(g[e], h[e], c[e]);
+            }
+#pragma unroll
+            for (int o = N / 2; o >= 1; o >>= 1)
+#pragma unroll
+                for (int e = 0; e < o; e++) c[e] += c[e + o];
+            const float mean = row_sum(c[0], tpr, lds, turn) / (float)a.F;
+            if (a.ds == nullptr) continue;
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int at = (t + k * tpr) * N;
+                if (at >= a.F) continue;
+                float h[N], g[N];
+                terms(k, h, g);
+                times_gain(at, g);
+#pragma unroll
+                for (int e = 0; e < N; e++) g[e] = rstd * (g[e] - h[e] * mean);
+                if (a.gs) {
+                    raw_float<T, N>(raw_use<T, N, FIT>(sq[k], at, a.F), h);
+#pragma unroll
+                    for (int e = 0; e < N; e++) g[e] += h[e];
+                }
+                row_store<T, N, FIT, NT>((T*)a.ds + i * a.F, at, a.F, g);
+            }
+            continue;
+        }
         const float rs = rstd;
         float h[NV][N], g[NV][N], c[N];
         V q[NV];
@@ -564,7 +628,7 @@ template <class T, int NV, int FIT, bool NT, int MOST> __global__ __launch_bound
                 for (int e = 0; e < N; e++) h[k][e] += r[e];
             }
         }
-        if (AHEAD) fetch(i + step);             // in flight while this row is reduced and written
+        fetch(i + step);                        // in flight while this row is reduced and written
 #pragma unroll
         for (int e = 0; e < N; e++) c[e] = 0.0f;
         // (a vector behind the row holds zeros; a row that is off holds an earlier one and has no part in dw)

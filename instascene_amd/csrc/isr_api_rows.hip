@@ -42,7 +42,7 @@ RowShape row_shape(int vecs, long long rows, int least, int max_nv, int max_wave
     if (per_lane <= (tsh == 6 && rows * 64 < 256 * 256 ? 1 : 2)) return {1 << tsh, (1 << tsh) - 1, tsh, 256 >> tsh, per_lane, 256};
     for (int nv = rows * ((vecs + 1) / 2) < 256 * 256 ? 1 : 2; nv <= max_nv; nv *= 2) {
         const int waves = (vecs + 64 * nv - 1) / (64 * nv);
-        if (waves <= max_waves) return {64 * waves, 0x7fffffff, 31, 1, nv, 64 * waves};
+        if (waves <= (nv == max_nv ? max_waves : 8)) return {64 * waves, 0x7fffffff, 31, 1, nv, 64 * waves};
     }
     return {512, 0x7fffffff, 31, 1, 0, 512};
 }
@@ -88,7 +88,7 @@ void launch_codes(int code, int type, const iso::RmsArgs& a, hipStream_t s) {
 // workgroups of the backward pass = partial rows of dw: enough to keep the memory busy (two of 256 threads per compute unit do for wide rows:
 // 768 and 1024 workgroups took 1 to 14 % longer at [n, 2048..4096] float32), few enough that the partials stay small against the rows
 template <class T> RowShape backward_shape(long long rows, int F, int& grid) {
-    const RowShape sh = row_shape((F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, rows, 1, 2, sizeof(T) == 4 ? 16 : 8);       // (what the registers hold)
+    const RowShape sh = row_shape((F + iso::RowVec<T>::N - 1) / iso::RowVec<T>::N, rows, 1, 2, 16);       // (what the registers hold)
     if (sh.nv == 0) {           // slices of the columns' sums: 1024 workgroups with those that the columns need
         const int cols = 256 * iso::RowVec<T>::N;
         grid = (int)std::max<long long>(1, std::min<long long>(rows, std::max(16, 1024 / ((F + cols - 1) / cols))));
@@ -102,9 +102,9 @@ RowShape backward_shape_type(int type, long long rows, int F, int& grid) {
     return type == 0 ? backward_shape<float>(rows, F, grid) : type == 1 ? backward_shape<__bf16>(rows, F, grid) : backward_shape<_Float16>(rows, F, grid);
 }
 template <class T, int FIT, bool NT> void launch_backward_fit(const iso::RmsBackArgs& a, int nv, int block, int grid, hipStream_t s) {
-    if (nv == 1) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 1, FIT, NT, 512>), dim3(grid), dim3(block), 0, s, a);
-    else if (block <= 512) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 2, FIT, NT, 512>), dim3(grid), dim3(block), 0, s, a);
-    else if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 2, FIT, NT, 1024>), dim3(grid), dim3(block), 0, s, a);
+    if (block > 512) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 2, FIT, NT, 1024>), dim3(grid), dim3(block), 0, s, a);
+    else if (nv == 1) hipLaunchKernelGGL((iso::rms_backward_kernel<T, 1, FIT, NT, 512>), dim3(grid), dim3(block), 0, s, a);
+    else hipLaunchKernelGGL((iso::rms_backward_kernel<T, 2, FIT, NT, 512>), dim3(grid), dim3(block), 0, s, a);
 }
 template <class T> void launch_backward(iso::RmsBackArgs a, int nv, int block, int grid, hipStream_t s) {
     if (nv != 0) {

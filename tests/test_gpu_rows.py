@@ -40,7 +40,7 @@ def check(got, want, tol, name):
 
 
 # one column to long rows: below / at / above a vector, a wave, a workgroup, the registers (16 384 float32, 32 768 of 16 bits)
-WIDTHS = [1, 3, 4, 8, 31, 32, 63, 64, 65, 255, 256, 1021, 1024, 2048, 4097, 8192, 16384, 16385, 33000]
+WIDTHS = [1, 3, 4, 8, 31, 32, 63, 64, 65, 255, 256, 1021, 1024, 2048, 2052, 2943, 4096, 4097, 6000, 8192, 8200, 9001, 16384, 16385, 33000]
 
 
 def norm_reference(x, w, eps, r):
