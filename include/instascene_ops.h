@@ -253,7 +253,7 @@ int iso_rows8_read(int type, int code, long long n, int F, int group, long long 
 /* The norm of all elements of `count` tensors together - norm_type 2, 1, or 0 for the largest magnitude - and, with clip, their scaling in
  * place:  out[0] = norm,  out[1] = coef = min(1, max_norm / (norm + 1e-6)),  tensor *= coef (left alone where coef is 1).
  * tensors / sizes / types are HOST arrays; a size may be 0; with clip no two tensors may share memory.  Sums are held in 64 bits, in an order
- * that the sizes alone fix.  scratch: iso_grad_norm_scratch_bytes of device memory. */
+ * that the sizes and the tensors' alignment fix.  scratch: iso_grad_norm_scratch_bytes of device memory. */
 size_t iso_grad_norm_scratch_bytes(int count, const long long* sizes);
 int iso_grad_norm(int count, void* const* tensors, const long long* sizes, const int* types, int norm_type, float max_norm, int clip,
                   float* out /*[2]*/, void* scratch, size_t scratch_bytes, void* stream);

@@ -6,7 +6,7 @@
 // (a whole launch leaves after it has read the partial sums).  The tensors are cut into chunks of GN_CHUNK elements; a table of at
 // most GN_TENSORS tensors travels in the kernel's arguments, so that no copy to the device precedes a launch and a captured graph holds
 // all of it.  Workgroup b sums chunks b, b + grid, ... in 64 bits (no overflow, and long sums lose nothing) into partial b: no atomics, the
-// order of every sum is fixed by the sizes alone.  The scaling kernel's workgroups each add the partials up for themselves (at most
+// order of every sum is fixed by the sizes and alignments alone.  The scaling kernel's workgroups each add the partials up for themselves (at most
 // GN_PARTS of them, from L2) instead of waiting for a launch of their own that does.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -197,7 +197,8 @@ __global__ __launch_bounds__(GN_THREADS) void gaussian_norm_kernel(GaussNormArgs
             norm_add<2>(acc, a.scale[2 * i + 1] * expf(a.p_scale[2 * i + 1]));
         }
         if (a.rot) {
-            const float4 q = reinterpret_cast<const float4*>(a.p_rot)[i], g = reinterpret_cast<const float4*>(a.rot)[i];
+            typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+            const V q = reinterpret_cast<const V*>(a.p_rot)[i], g = reinterpret_cast<const V*>(a.rot)[i];
             const float n = fmaxf(__builtin_sqrtf(q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w), 1e-12f), r = 1.0f / n;
             const float4 y = make_float4(q.x * r, q.y * r, q.z * r, q.w * r);
             const float d = y.x * g.x + y.y * g.y + y.z * g.z + y.w * g.w;

@@ -7,8 +7,8 @@
 //   backward:  h = s rstd,  c = mean(gy w h),  ds = rstd (gy w - h c) + gs,  dw = sum over rows of gy h
 //
 // All of it is bound by memory: every element is read once, kept in registers between the reduction and the output, and
-// written once.  `tpr` threads (a power of two) share a row, NV vectors of 16 input bytes each, vector j = t + k tpr, so
-// that a wave's loads are contiguous; rows longer than the registers hold are read a second time (the *_long kernels).
+// written once.  `tpr` threads share a row (a power of two up to a wave, beyond it a workgroup of whole waves), NV vectors of 16 input bytes
+// each, vector j = t + k tpr, so that a wave's loads are contiguous; rows longer than the registers hold are read a second time (the *_long kernels).
 // Sums of squares are held in 32 bits, in short chains (a vector's elements side by side, then a tree); a row whose sum leaves
 // [1e-30, 1e37] is summed again in 64 bits, so that no finite row overflows or vanishes.  (64 bits throughout cost a quarter of the time of
 // narrow rows: conversions and 64-bit additions run at a fraction of the rate.)
@@ -187,8 +187,8 @@ __device__ __forceinline__ unsigned row_max(unsigned v, int tpr, double (*lds)[1
     }
     return v;
 }
-// The sum of squares of a row of which this thread holds v[NV][N]; `on`: the row is one (the others may be anything).  Returned as
-// (fast, wide): wide < 0 where the 32-bit sum is good.  The test is the same in all threads of a row; a wave that shares several rows
+// The sum of squares of a row of which this thread holds v[NV][N]; `on`: the row is one (the others may be anything).  Where the 32-bit sum
+// is no good the 64-bit one is in `wide` (else wide < 0).  The test is the same in all threads of a row; a wave that shares several rows
 // repeats the sum for all of them.
 template <int NV, int N> __device__ __forceinline__ float row_squares(const float (&v)[NV][N], bool on, int tpr, double (*lds)[16], double& wide) {
     float acc[N];

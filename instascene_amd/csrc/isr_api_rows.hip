@@ -369,7 +369,6 @@ int iso_gaussian_grad_norm(int P, int M, float* const params[6], const float* g_
     if (!params || !out || !(max_norm >= 0.0f)) return fail(ISR_EINVAL, "gaussian_grad_norm: null argument, or max_norm negative");
     if (!scratch || scratch_bytes < iso_grad_norm_scratch_bytes(1, nullptr)) return fail(ISR_EINVAL, "gaussian_grad_norm: scratch too small");
     if (P > 0 && ((g_opacity && !params[3]) || (g_scale && !params[4]) || (g_rotation && !params[5]))) return fail(ISR_EINVAL, "gaussian_grad_norm: a gradient without its parameter");
-    if (((uintptr_t)g_rotation | (g_rotation ? (uintptr_t)params[5] : 0)) & 15) return fail(ISR_EINVAL, "gaussian_grad_norm: rotations must be 16-byte aligned");
     double* part = (double*)scratch;
     int parts = 0;
     if (P > 0) {
