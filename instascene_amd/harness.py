@@ -280,7 +280,8 @@ class SegTrainer:
 
     def features_in_input_order(self) -> torch.Tensor:
         """The trained ``[P,F]`` feature with rows in the order of the scene passed to the constructor."""
-        f = self.model._seg_feature.detach()
+        f = self.model._seg_feature
+        f = f.read() if isinstance(f, QuantizedRows) else f.detach()         # (compact_features: the values of the 8-bit rows)
         if self.order is None:
             return f.clone()
         out = torch.empty_like(f)

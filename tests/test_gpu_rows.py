@@ -346,6 +346,25 @@ def test_table_ranges_strides_and_state():
     assert bool((t.read(torch.tensor([-1], device="cuda"), norm_eps=0.0) == 0).all())
 
 
+def test_one_row_without_a_row_dimension_and_other_index_forms():
+    import numpy as np
+    x = make((300,), BF16, 1)
+    assert torch.equal(rms_norm(x), rms_norm(x[None])[0])
+    leaf = x.clone().requires_grad_(True)
+    dx, = torch.autograd.grad(rms_norm(leaf), leaf, x)
+    deep = x[None, None].clone().requires_grad_(True)
+    d3, = torch.autograd.grad(rms_norm(deep), deep, x[None, None])
+    assert dx.shape == (300,) and torch.equal(dx, d3[0, 0])
+    t = QuantizedRows(9, 300, dtype=torch.int8)
+    t.write(x[None], np.int64(4))
+    assert torch.equal(t.read(slice(4, 5)), QuantizedRows.from_rows(x[None], dtype=torch.int8).read()) and bool((t.read(slice(5, 9)) == 0).all())
+    every_second = torch.arange(18, device="cuda")[::2]                     # an index with a stride
+    assert torch.equal(t.read(every_second.flip(0)), torch.cat((torch.zeros(4, 300, device="cuda"), t.read(every_second.flip(0)[4:]))))
+    assert torch.equal(t.read(every_second)[2], t.read(slice(4, 5))[0])
+    with pytest.raises(TypeError):
+        t.write(x[None], 4.0)
+
+
 def test_offsets_beyond_32_bits():
     """More than 2^32 code bytes, more than 2^31 elements of a norm."""
     P, F = 68_000_000, 64
@@ -501,6 +520,17 @@ def test_a_trained_table_in_8_bits_renders(code, group):
               + 2.0 ** -10 * rows.double().abs().amax(1, keepdim=True) / 448 + 4 * U, "codes")
         with pytest.raises(RuntimeError):
             m.compact_features()
+
+
+def test_a_trainer_hands_out_its_compacted_features_in_input_order():
+    from instascene_amd import scenes
+    from instascene_amd.harness import SegTrainer
+    sc = scenes.synthetic_scene(2000, 16, 5, math.log(0.04))
+    t = SegTrainer(sc, scenes.ring_cameras(6, 96, 64), device="cuda", sample_batchsize=512, n_labels=8, use_class_feat=True, seed=3)
+    t.step(0)
+    want = row_normalize(t.features_in_input_order(), 1e-6)
+    t.model.compact_features(torch.int8)
+    check(t.features_in_input_order(), want.double(), want.double().abs().amax(1, keepdim=True) * (0.5 / 127 + 4 * U), "input order")
 
 
 def test_a_residual_table_is_trained_clipped_and_put_away():
