@@ -4,11 +4,14 @@
 // Errors: TypeError / ValueError for arguments, instascene_amd._lib.IsrError for what the library refuses.
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <limits>
 #include <optional>
 #include <stdexcept>
@@ -34,6 +37,22 @@ int row_type(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16
 int code_type(at::ScalarType t) { return t == at::kChar ? 1 : t == at::kFloat8_e4m3fn ? 2 : 0; }
 
 constexpr int64_t MAX_WIDTH = 1 << 24;
+
+// The kernels write through raw pointers, which a trace does not record (what it would keep is the uninitialised output) and which carry no
+// tangent: both are refused, by every entry, before anything else is looked at.
+void refuse_trace(const char* what) {
+    using c10::impl::TorchDispatchModeKey;
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value(), what,
+                " cannot be traced: its kernels would not be recorded");
+}
+void refuse_tangent(const char* what, const Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative, and an input carries a tangent");
+}
+void refuse_modes(const char* what, std::initializer_list<OptTensor> inputs) {
+    refuse_trace(what);
+    for (const OptTensor& t : inputs)
+        if (t) refuse_tangent(what, *t);
+}
 
 void check_rows(const char* what, const Tensor& x) {
     TORCH_CHECK(x.is_cuda(), what, ": needs CUDA tensors (the HIP library is the only backend)");
@@ -137,6 +156,7 @@ private:
         const bool need_x = ctx->saved_data["x"].toBool(), need_w = ctx->saved_data["w"].toBool(), need_r = ctx->saved_data["r"].toBool();
         if (!gy.defined())                                      // only the sum was used: its gradient passes through
             return {need_x ? gs : Tensor(), Tensor(), Tensor(), need_r ? gs : Tensor()};
+        refuse_modes("the backward pass of rms_norm", {gy, gs});
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2], &rstd = saved[3];
         const c10::DeviceGuard guard(x.device());
@@ -166,6 +186,7 @@ bool wants_grad(const Tensor& x, const OptTensor& weight, const OptTensor& resid
 
 // (y, s), s None without a residual
 std::pair<Tensor, OptTensor> rms_norm(const Tensor& x, const OptTensor& weight, double eps, const OptTensor& residual) {
+    refuse_modes("rms_norm", {x, weight, residual});
     check_norm("rms_norm", x, weight, eps, residual);
     if (wants_grad(x, weight, residual)) {
         auto out = RmsNorm::apply(x, weight, eps, residual);
@@ -179,6 +200,7 @@ std::pair<Tensor, OptTensor> rms_norm(const Tensor& x, const OptTensor& weight, 
 std::tuple<Tensor, Tensor, OptTensor> rms_norm_quantized(const Tensor& x, const OptTensor& weight_, double eps, const OptTensor& residual_,
                                                          at::ScalarType dtype, std::optional<int64_t> group) {
     const char* what = "rms_norm_quantized";
+    refuse_modes(what, {x, weight_, residual_});
     check_norm(what, x, weight_, eps, residual_);
     TORCH_CHECK_VALUE(x.dim() == 2, what, ": x must be [rows, F]");
     const int code = check_code(what, dtype);
@@ -205,6 +227,7 @@ Tensor check_index(const char* what, const Tensor& index, const Tensor& codes, i
 // rows into the table: `index` (with `owner` beyond ISO_ROWS8_SCAN of them), or the rows from `first` on
 void rows8_write(const Tensor& codes, const Tensor& scales, const OptTensor& owner, const Tensor& rows, const OptTensor& index, int64_t first) {
     const char* what = "QuantizedRows.write";
+    refuse_modes(what, {rows});
     const int64_t P = codes.size(0), F = codes.size(1);
     check_rows(what, rows);
     TORCH_CHECK_VALUE(rows.dim() == 2 && rows.size(1) == F && rows.device() == codes.device(), what, ": rows must be [n, ", F, "] on ", codes.device(), ", not ",
@@ -225,6 +248,7 @@ void rows8_write(const Tensor& codes, const Tensor& scales, const OptTensor& own
 Tensor rows8_read(const Tensor& codes, const Tensor& scales, const OptTensor& index, int64_t first, int64_t count, at::ScalarType out_dtype,
                   std::optional<double> norm_eps) {
     const char* what = "QuantizedRows.read";
+    refuse_trace(what);
     const int type = row_type(out_dtype);
     TORCH_CHECK_TYPE(type >= 0, what, ": out_dtype must be float32, bfloat16 or float16, not ", out_dtype);
     TORCH_CHECK_VALUE(!norm_eps || (*norm_eps >= 0.0 && std::isfinite((float)*norm_eps)), what, ": norm_eps must be finite and not negative");
@@ -246,6 +270,8 @@ bool is_dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlappin
 // (norm, factor) of all elements together [, and the tensors scaled in place]
 Tensor norm_and_factor(const std::vector<Tensor>& tensors, double norm_type, double max_norm, bool clip) {
     const char* what = clip ? "clip_grads_" : "grad_norm";
+    refuse_trace(what);
+    for (const Tensor& t : tensors) refuse_tangent(what, t);
     const int kind = norm_type == 2.0 ? 2 : norm_type == 1.0 ? 1 : norm_type == std::numeric_limits<double>::infinity() ? 0 : -1;
     TORCH_CHECK_VALUE(kind >= 0, what, ": norm_type must be 1, 2 or inf, not ", norm_type);
     const at::AutoGradMode off(false);
