@@ -267,6 +267,75 @@ Tensor rows8_read(const Tensor& codes, const Tensor& scales, const OptTensor& in
 // one stretch of memory, each element once (in any order of the dimensions)
 bool is_dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
 
+// Memory that strided tensors share, decided on the host: a byte of `a` is a byte of `b` where  sum stride_k x_k = address(a) - address(b)  has a
+// solution in whole numbers, with the indices of b counted up, those of a counted down and a byte within an element as one more dimension.
+struct Dim { int64_t stride, lo, hi; };
+int64_t floor_div(int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); }
+// dims by falling stride.  Nested strides, as views have them, leave two or three candidates per dimension; a search that does not end within
+// `left` steps (strides that no view of a bucket has) counts as shared.
+bool reaches(const std::vector<Dim>& dims, size_t k, int64_t target, int& left) {
+    if (k == dims.size()) return target == 0;
+    if (--left < 0) return true;
+    int64_t least = 0, most = 0;                // what the smaller strides reach
+    for (size_t j = k + 1; j < dims.size(); j++) { least += dims[j].stride * dims[j].lo; most += dims[j].stride * dims[j].hi; }
+    const int64_t s = dims[k].stride, from = std::max(dims[k].lo, -floor_div(most - target, s)), to = std::min(dims[k].hi, floor_div(target - least, s));
+    for (int64_t x = from; x <= to; x++)
+        if (reaches(dims, k + 1, target - s * x, left)) return true;
+    return false;
+}
+void add_dims(std::vector<Dim>& dims, const Tensor& t, bool up, bool down) {
+    auto add = [&](int64_t stride, int64_t n) {
+        for (Dim& d : dims)
+            if (d.stride == stride) { d.lo -= down ? n : 0; d.hi += up ? n : 0; return; }
+        dims.push_back({stride, down ? -n : 0, up ? n : 0});
+    };
+    const int64_t size = t.element_size();
+    add(1, size - 1);
+    for (int64_t i = 0; i < t.dim(); i++)
+        if (t.size(i) > 1) add(t.stride(i) * size, t.size(i) - 1);
+}
+constexpr int SEARCH = 100000;
+void by_stride(std::vector<Dim>& dims) { std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; }); }
+bool share_memory(const Tensor& a, const Tensor& b) {
+    std::vector<Dim> dims;
+    add_dims(dims, a, false, true);
+    add_dims(dims, b, true, false);
+    by_stride(dims);
+    int left = SEARCH;
+    return reaches(dims, 0, (int64_t)((intptr_t)a.data_ptr() - (intptr_t)b.data_ptr()), left);
+}
+// two elements of one tensor in one place (strides that are not 0)
+bool overlaps_itself(const Tensor& t) {
+    const int64_t size = t.element_size();
+    int left = SEARCH;
+    for (int64_t i = 0; i < t.dim(); i++) {
+        if (t.size(i) <= 1) continue;
+        std::vector<Dim> dims;
+        add_dims(dims, t.select(i, 0), true, true);
+        dims.push_back({t.stride(i) * size, 1, t.size(i) - 1});
+        by_stride(dims);
+        if (reaches(dims, 0, 0, left)) return true;
+    }
+    return false;
+}
+void refuse_shared_memory(const std::vector<Tensor>& tensors) {
+    struct Span { uintptr_t from, to; const Tensor* t; bool dense; };
+    std::vector<Span> spans;
+    for (const Tensor& t : tensors) {
+        if (t.numel() == 0) continue;
+        int64_t reach = 1;
+        for (int64_t d = 0; d < t.dim(); d++) reach += (t.size(d) - 1) * t.stride(d);
+        const uintptr_t from = (uintptr_t)t.data_ptr();
+        spans.push_back({from, from + (uintptr_t)(reach * (int64_t)t.element_size()), &t, is_dense(t)});
+        if (!spans.back().dense && overlaps_itself(t)) throw LibraryError("clip_grads_: a tensor to be clipped has elements that share memory");
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+    for (size_t i = 0; i < spans.size(); i++)
+        for (size_t j = i + 1; j < spans.size() && spans[j].from < spans[i].to; j++)
+            if ((!spans[i].dense || !spans[j].dense) && share_memory(*spans[i].t, *spans[j].t))
+                throw LibraryError("clip_grads_: two of the tensors to be clipped share memory");
+}
+
 // (norm, factor) of all elements together [, and the tensors scaled in place]
 Tensor norm_and_factor(const std::vector<Tensor>& tensors, double norm_type, double max_norm, bool clip) {
     const char* what = clip ? "clip_grads_" : "grad_norm";
@@ -298,6 +367,7 @@ Tensor norm_and_factor(const std::vector<Tensor>& tensors, double norm_type, dou
         sizes[i] = t.numel();
         types[i] = row_type(t.scalar_type());
     }
+    if (clip && !copies.empty()) refuse_shared_memory(tensors);        // (the library sees the copies' addresses)
     const c10::DeviceGuard guard(dev);
     const size_t bytes = iso_grad_norm_scratch_bytes(n, sizes.data());
     const auto opts = tensors[0].options().memory_format(std::nullopt);
