@@ -2,7 +2,7 @@
 addition (:func:`rms_norm`, with its backward pass), the same with an output in 8 bits (:func:`rms_norm_quantized`), and a table kept in
 8 bits (:class:`QuantizedRows`: written as a whole, by range or by index, read back likewise).  The kernels are ``iso_rms_norm_*``
 and ``iso_rows8_*`` (include/instascene_ops.h); every call runs on the current stream of its tensors' device, allocates from torch and
-synchronises nothing, so it can be captured into a graph."""
+synchronises nothing (but see :meth:`QuantizedRows.write`), so it can be captured into a graph."""
 from __future__ import annotations
 
 import functools
@@ -105,7 +105,9 @@ class QuantizedRows:
     def write(self, rows: torch.Tensor, index=None) -> "QuantizedRows":
         """Quantise ``rows [n, width]`` into the table: all of it (``index`` None, n = rows of the table), rows ``[index, index + n)`` (an
         int), or row ``index[i]`` for every i (an int64 or int32 tensor): of equal indices the last is kept, and an index outside the
-        table - the padding of a batch - writes nothing.  Other rows stay as they are."""
+        table - the padding of a batch - writes nothing.  Other rows stay as they are.  Two streams may write disjoint rows at once.  The
+        first write of more than 256 indices to a table of ``from_rows`` / ``rms_norm_quantized`` makes a helper table ``[rows]`` and waits
+        for it: the one synchronisation of this class."""
         what = "QuantizedRows.write"
         P = self.codes.shape[0]
         first, ix = 0, None
@@ -120,7 +122,10 @@ class QuantizedRows:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError(f"{what}: the first write of more than {SCAN_MAX} indices to this table makes a helper table and "
                                        "cannot be captured: write once before the capture")
-                self._owner = torch.full((P,), -1, dtype=torch.int32, device=self.codes.device)
+                owner = torch.full((P,), -1, dtype=torch.int32, device=self.codes.device)
+                # once per table: from here on any stream may write, also one that waits for nothing this stream has done
+                torch.cuda.current_stream(owner.device).synchronize()
+                self._owner = owner
         _ext().rows8_write(self.codes, self.scales, self._owner, rows, ix, first)
         return self
 
