@@ -145,6 +145,13 @@ class QuantizedRows:
             ix = index
         return _ext().rows8_read(self.codes, self.scales, ix, first, n, out_dtype, norm_eps)
 
+    def record_stream(self, stream) -> None:
+        """``torch.Tensor.record_stream`` for all of the table's memory, the helper table included: needed where the table is used on another
+        stream than the one it was made on and may be dropped before that stream is done."""
+        for t in (self.codes, self.scales, self._owner):
+            if t is not None:
+                t.record_stream(stream)
+
     def state_dict(self):
         return {"codes": self.codes, "scales": self.scales}
 

@@ -33,3 +33,26 @@ def test_a_second_stream_writes_right_behind_the_first_large_write():
         want[a], want[b] = QuantizedRows.from_rows(xa, dtype=torch.int8).read(), QuantizedRows.from_rows(xb, dtype=torch.int8).read()
         assert torch.equal(t.read(), want), k
         assert bool((t._owner == -1).all())
+
+
+def test_a_dropped_table_stays_until_the_other_stream_is_done():
+    P, F = 300_000, 32
+    x, index = torch.randn(1000, F, device="cuda"), torch.arange(1000, device="cuda")
+    t = QuantizedRows(P, F, dtype=torch.int8)
+    busy = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy = torch.tanh(busy @ busy)
+        t.write(x, index)
+    t.record_stream(side)
+    held = {m.data_ptr() for m in (t.codes, t.scales, t._owner)}
+    done = torch.cuda.Event()
+    done.record(side)
+    del t
+    fresh = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in (P * F, 4 * P, 4 * P)]
+    if done.query():
+        pytest.skip("the other stream was done too early to tell")
+    assert not held & {m.data_ptr() for m in fresh}
+    torch.cuda.synchronize()
