@@ -226,7 +226,8 @@ int iso_rms_norm_forward(int type, long long rows, int F, const void* x, long lo
                          float* rstd /*[rows]*/, void* stream);
 /* The same with y in 8 bits: codes [rows, F] (code 1: int8, 2: e4m3), scales [rows, F / group]; y is about code * scale.  Per group of
  * `group` columns (F, or 32 / 64 / 128 dividing F): top = max |s weight|, code = s weight Q / top to the nearest, ties to even,
- * scale = top rstd / Q, Q = 127 (int8) or 448 (e4m3).  Groups below 2^-116 are zeros; a group with an infinity or NaN has scale NaN. */
+ * scale = top rstd / Q, Q = 127 (int8) or 448 (e4m3).  Groups whose top is below 2^-116 are zeros; a group in which s or weight holds an
+ * infinity or NaN has scale NaN (a product s weight beyond the largest float is kept: y is finite). */
 int iso_rms_norm_quant(int type, int code, long long rows, int F, int group, const void* x, long long x_stride, const void* residual,
                        long long residual_stride, const void* weight, int weight_is_float, float eps, void* codes, float* scales,
                        void* s_out, void* stream);

@@ -322,6 +322,17 @@ template <int N> __device__ __forceinline__ unsigned top_bits_of(const float (&v
     return m;
 }
 
+// s w beyond the largest float although s is finite: the vector is loaded again and formed as (s 2^-64) (w 2^-65), its scale times 2^129.  The
+// scaling changes no code: what it loses to small numbers lies below top 2^-20, whose code is 0.  Rare, so behind a branch that whole waves take.
+constexpr unsigned BEYOND = 0x7f800000u;
+template <int N> __device__ __forceinline__ void scaled_product(const float (&s)[N], const float (&w)[N], float (&v)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; e++) v[e] = (s[e] * 0x1p-64f) * (w[e] * 0x1p-65f);
+}
+__device__ __forceinline__ float stored_scale(float scale, float rstd, bool scaled) {
+    return scaled ? (float)((double)scale * (double)rstd * 0x1p129) : scale * rstd;
+}
+
 // ---- where a written row goes ----------------------------------------------------------------------------------------------------
 // index == NULL: row first + i.  Otherwise row index[i]; of equal indices the last one is kept, indices outside [0, P) write nothing.
 // owner == NULL: the row looks through the entries behind it (few rows).  owner [P], all -1 between calls: row_claim_kernel has left
@@ -414,23 +425,53 @@ template <class T, int NV, int OUT, int FIT, bool NT> __global__ __launch_bounds
     if constexpr (OUT != 0) {
         const long long row = row_target(a.to, i, a.rows, t, tpr, lds);
         const int seg = a.groups == 1 ? 0 : (1 << a.gshift) / N;
+        auto again = [&](int k) {
+            const int at = (t + k * tpr) * N;
+            float s[N], w[N];
+            sum_load<T, N, FIT>(x, res, at, a.F, on, s);
+#pragma unroll
+            for (int e = 0; e < N; e++) w[e] = 0.0f;
+            if (at < a.F) gain_load<T, N, FIT>(a.w, a.w32, at, a.F, w);
+            scaled_product(s, w, v[k]);
+        };
         unsigned top = 0;
+        bool scaled = false;
         if (seg == 0) {
 #pragma unroll
             for (int k = 0; k < NV; k++) top = max(top, top_bits_of(v[k]));
             top = row_max(top, tpr, lds, 1);
+            scaled = top >= BEYOND;
+            if (__any(scaled)) {                    // (tpr > 64: one row, all of its waves agree)
+                unsigned small = 0;
+#pragma unroll
+                for (int k = 0; k < NV; k++) {
+                    if (scaled) again(k);
+                    small = max(small, top_bits_of(v[k]));
+                }
+                if (tpr > 64) __syncthreads();      // slot 1 has been read by everybody
+                small = row_max(small, tpr, lds, 1);
+                if (scaled) top = small;
+            }
         }
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int at = (t + k * tpr) * N;
-            if (seg != 0) top = lanes_max(top_bits_of(v[k]), seg);          // a group's vectors lie in `seg` neighbouring lanes of one wave
+            if (seg != 0) {                         // a group's vectors lie in `seg` neighbouring lanes of one wave
+                top = lanes_max(top_bits_of(v[k]), seg);
+                scaled = top >= BEYOND;
+                if (__any(scaled)) {
+                    if (scaled) again(k);
+                    const unsigned small = lanes_max(top_bits_of(v[k]), seg);
+                    if (scaled) top = small;
+                }
+            }
             const Group8 g = group_scale<OUT>(top);
             if (row < 0 || at >= a.F) continue;
             unsigned c[N / 4];
 #pragma unroll
             for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[k][4 * q], g);
             code_store<N, FIT>(a.codes + row * a.F, at, a.F, c);
-            if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
+            if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = stored_scale(g.scale, rstd, scaled);
         }
     }
 }
@@ -462,6 +503,19 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
     float rstd = 1.0f;
     if (a.norm) rstd = rms_inverse(0.0f, row_sum(ss, tpr, lds, 0), a.inv_F, a.eps);
     if (by_row) row_top = row_max(row_top, tpr, lds, 1);
+    const bool row_scaled = by_row && row_top >= BEYOND;
+    if (row_scaled) {                           // (the workgroup is the row)
+        row_top = 0;
+        for (int at = t * N; at < a.F; at += tpr * N) {
+            float v[N], w[N];
+            sum_load<T, N, TAIL>(x, res, at, a.F, true, v);
+            gain_load<T, N, TAIL>(a.w, a.w32, at, a.F, w);
+            scaled_product(v, w, v);
+            row_top = max(row_top, top_bits_of(v));
+        }
+        __syncthreads();                        // slot 1 has been read by everybody
+        row_top = row_max(row_top, tpr, lds, 1);
+    }
     if (a.rstd && t == 0) a.rstd[i] = rstd;
     const int seg = OUT == 0 || by_row ? 0 : (1 << a.gshift) / N;
     // (all threads of a wave take every step together: the groups' maxima go from lane to lane)
@@ -474,18 +528,32 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
 #pragma unroll
         for (int e = 0; e < N; e++) w[e] = 0.0f;
         if (in) gain_load<T, N, TAIL>(a.w, a.w32, at, a.F, w);
-#pragma unroll
-        for (int e = 0; e < N; e++) v[e] = OUT == 0 ? v[e] * rstd * w[e] : v[e] * w[e];
         if constexpr (OUT == 0) {
+#pragma unroll
+            for (int e = 0; e < N; e++) v[e] = v[e] * rstd * w[e];
             if (in) row_store<T, N, TAIL>((T*)a.y + i * a.F, at, a.F, v);
         } else {
-            const Group8 g = group_scale<OUT>(seg != 0 ? lanes_max(top_bits_of(v), seg) : row_top);
+            float s[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) { s[e] = v[e]; v[e] *= w[e]; }
+            unsigned top = row_top;
+            bool scaled = row_scaled;
+            if (seg != 0) {
+                top = lanes_max(top_bits_of(v), seg);
+                scaled = top >= BEYOND;
+            }
+            if (__any(scaled)) {
+                if (scaled) scaled_product(s, w, v);
+                const unsigned small = seg != 0 ? lanes_max(top_bits_of(v), seg) : row_top;
+                if (scaled) top = small;
+            }
+            const Group8 g = group_scale<OUT>(top);
             if (row >= 0 && in) {
                 unsigned c[N / 4];
 #pragma unroll
                 for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[4 * q], g);
                 code_store<N, TAIL>(a.codes + row * a.F, at, a.F, c);
-                if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = g.scale * rstd;
+                if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = stored_scale(g.scale, rstd, scaled);
             }
         }
     }

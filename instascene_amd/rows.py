@@ -41,8 +41,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
 
 def rms_norm_quantized(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
                        dtype: torch.dtype = torch.float8_e4m3fn, group: Optional[int] = None):
-    """:func:`rms_norm` of ``[rows, F]`` with the output in 8 bits: a :class:`QuantizedRows`, or ``(rows, s)`` with a residual.  Not
-    differentiable: inputs that require a gradient are refused unless gradients are disabled."""
+    """:func:`rms_norm` of ``[rows, F]`` with the output in 8 bits: a :class:`QuantizedRows`, or ``(rows, s)`` with a residual.  The codes are
+    those of ``s * weight``: a group of which that stays below 2^-116 everywhere is stored as zeros.  Not differentiable: inputs that require a gradient are refused unless gradients are disabled."""
     codes, scales, s = _ext().rms_norm_quantized(x, weight, eps, residual, dtype, group)
     out = QuantizedRows._of(codes, scales)
     return out if s is None else (out, s)
