@@ -323,7 +323,8 @@ template <int N> __device__ __forceinline__ unsigned top_bits_of(const float (&v
 }
 
 // s w beyond the largest float although s is finite: the vector is loaded again and formed as (s 2^-64) (w 2^-65), its scale times 2^129.  The
-// scaling changes no code: what it loses to small numbers lies below top 2^-20, whose code is 0.  Rare, so behind a branch that whole waves take.
+// scaling changes no code: what it loses to small numbers lies below top 2^-20, whose code is 0.  Rare, so behind a branch that whole
+// waves take.
 constexpr unsigned BEYOND = 0x7f800000u;
 template <int N> __device__ __forceinline__ void scaled_product(const float (&s)[N], const float (&w)[N], float (&v)[N]) {
 #pragma unroll
@@ -392,8 +393,9 @@ struct RmsArgs {
     float* scales;          // [P, groups]
     RowTarget to;
 };
-// NT: the rows are read past the caches.
-template <class T, int NV, int OUT, int FIT, bool NT> __global__ __launch_bounds__(512) void rms_forward_kernel(RmsArgs a) {
+// NT: the rows are read past the caches.  GAIN (8 bits): there is one, so that a product may leave the floats (whose rare branch costs the
+// writing of a table, which has no gain, 4 %: 258 us for [5 M, 64], 269 with it).
+template <class T, int NV, int OUT, int FIT, bool NT, bool GAIN> __global__ __launch_bounds__(512) void rms_forward_kernel(RmsArgs a) {
     constexpr int N = RowVec<T>::N;
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x & a.mask;
@@ -416,62 +418,71 @@ template <class T, int NV, int OUT, int FIT, bool NT> __global__ __launch_bounds
         const int at = (t + k * tpr) * N;
         if (at >= a.F || !on) continue;
         if (a.s) row_store<T, N, FIT>((T*)a.s + i * a.F, at, a.F, v[k]);
-        float w[N];
-        gain_load<T, N, FIT>(a.w, a.w32, at, a.F, w);
+        if constexpr (OUT == 0 || GAIN) {
+            float w[N];
+            gain_load<T, N, FIT>(a.w, a.w32, at, a.F, w);
 #pragma unroll
-        for (int e = 0; e < N; e++) v[k][e] = OUT == 0 ? v[k][e] * rstd * w[e] : v[k][e] * w[e];
+            for (int e = 0; e < N; e++) v[k][e] = OUT == 0 ? v[k][e] * rstd * w[e] : v[k][e] * w[e];
+        }
         if constexpr (OUT == 0) row_store<T, N, FIT>((T*)a.y + i * a.F, at, a.F, v[k]);
     }
     if constexpr (OUT != 0) {
         const long long row = row_target(a.to, i, a.rows, t, tpr, lds);
         const int seg = a.groups == 1 ? 0 : (1 << a.gshift) / N;
-        auto again = [&](int k) {
-            const int at = (t + k * tpr) * N;
-            float s[N], w[N];
-            sum_load<T, N, FIT>(x, res, at, a.F, on, s);
-#pragma unroll
-            for (int e = 0; e < N; e++) w[e] = 0.0f;
-            if (at < a.F) gain_load<T, N, FIT>(a.w, a.w32, at, a.F, w);
-            scaled_product(s, w, v[k]);
-        };
-        unsigned top = 0;
-        bool scaled = false;
+        unsigned tops[NV], top = 0;
         if (seg == 0) {
 #pragma unroll
             for (int k = 0; k < NV; k++) top = max(top, top_bits_of(v[k]));
             top = row_max(top, tpr, lds, 1);
-            scaled = top >= BEYOND;
-            if (__any(scaled)) {                    // (tpr > 64: one row, all of its waves agree)
+#pragma unroll
+            for (int k = 0; k < NV; k++) tops[k] = top;
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; k++) {          // a group's vectors lie in `seg` neighbouring lanes of one wave
+                tops[k] = lanes_max(top_bits_of(v[k]), seg);
+                top = max(top, tops[k]);
+            }
+        }
+        bool scaled[NV] = {};
+        if constexpr (GAIN) {
+            auto again = [&](int k) {
+                const int at = (t + k * tpr) * N;
+                float s[N], w[N];
+                sum_load<T, N, FIT>(x, res, at, a.F, on, s);
+#pragma unroll
+                for (int e = 0; e < N; e++) w[e] = 0.0f;
+                if (at < a.F) gain_load<T, N, FIT>(a.w, a.w32, at, a.F, w);
+                scaled_product(s, w, v[k]);
+            };
+            if (__any(top >= BEYOND)) {             // (per row and tpr > 64: one row, all of its waves agree)
                 unsigned small = 0;
 #pragma unroll
                 for (int k = 0; k < NV; k++) {
-                    if (scaled) again(k);
+                    scaled[k] = tops[k] >= BEYOND;
+                    if (scaled[k]) again(k);
                     small = max(small, top_bits_of(v[k]));
                 }
-                if (tpr > 64) __syncthreads();      // slot 1 has been read by everybody
-                small = row_max(small, tpr, lds, 1);
-                if (scaled) top = small;
+                if (seg == 0) {
+                    if (tpr > 64) __syncthreads();  // slot 1 has been read by everybody
+                    small = row_max(small, tpr, lds, 1);
+                }
+#pragma unroll
+                for (int k = 0; k < NV; k++) {
+                    if (seg != 0) small = lanes_max(top_bits_of(v[k]), seg);
+                    tops[k] = scaled[k] ? small : tops[k];
+                }
             }
         }
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int at = (t + k * tpr) * N;
-            if (seg != 0) {                         // a group's vectors lie in `seg` neighbouring lanes of one wave
-                top = lanes_max(top_bits_of(v[k]), seg);
-                scaled = top >= BEYOND;
-                if (__any(scaled)) {
-                    if (scaled) again(k);
-                    const unsigned small = lanes_max(top_bits_of(v[k]), seg);
-                    if (scaled) top = small;
-                }
-            }
-            const Group8 g = group_scale<OUT>(top);
+            const Group8 g = group_scale<OUT>(tops[k]);
             if (row < 0 || at >= a.F) continue;
             unsigned c[N / 4];
 #pragma unroll
             for (int q = 0; q < N / 4; q++) c[q] = encode4<OUT>(&v[k][4 * q], g);
             code_store<N, FIT>(a.codes + row * a.F, at, a.F, c);
-            if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = stored_scale(g.scale, rstd, scaled);
+            if ((at & ((1u << a.gshift) - 1u)) == 0) a.scales[row * a.groups + (at >> a.gshift)] = stored_scale(g.scale, rstd, scaled[k]);
         }
     }
 }
@@ -503,7 +514,7 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
     float rstd = 1.0f;
     if (a.norm) rstd = rms_inverse(0.0f, row_sum(ss, tpr, lds, 0), a.inv_F, a.eps);
     if (by_row) row_top = row_max(row_top, tpr, lds, 1);
-    const bool row_scaled = by_row && row_top >= BEYOND;
+    const bool row_scaled = by_row && a.w && row_top >= BEYOND;
     if (row_scaled) {                           // (the workgroup is the row)
         row_top = 0;
         for (int at = t * N; at < a.F; at += tpr * N) {
@@ -540,9 +551,9 @@ template <class T, int OUT> __global__ __launch_bounds__(512) void rms_forward_l
             bool scaled = row_scaled;
             if (seg != 0) {
                 top = lanes_max(top_bits_of(v), seg);
-                scaled = top >= BEYOND;
+                scaled = a.w && top >= BEYOND;
             }
-            if (__any(scaled)) {
+            if (a.w && __any(scaled)) {
                 if (scaled) scaled_product(s, w, v);
                 const unsigned small = seg != 0 ? lanes_max(top_bits_of(v), seg) : row_top;
                 if (scaled) top = small;

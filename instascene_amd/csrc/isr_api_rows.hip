@@ -67,11 +67,16 @@ template <class T, int OUT> void launch_forward(iso::RmsArgs a, hipStream_t s) {
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
         const dim3 grid((unsigned)((n + rpb - 1) / rpb));
-#define FWD(NV, FIT) do { if (OUT != 0 && nt) hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, FIT, OUT != 0>), grid, dim3(block), 0, s, a); \
-                           else hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, FIT, false>), grid, dim3(block), 0, s, a); } while (0)
+#define FWD_AS(NV, FIT, NT, GAIN) hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, FIT, NT, GAIN>), grid, dim3(block), 0, s, a)
+#define FWD(NV, FIT) do { if (OUT == 0) FWD_AS(NV, FIT, false, false); \
+                           else if (nt && a.w) FWD_AS(NV, FIT, OUT != 0, OUT != 0); \
+                           else if (nt) FWD_AS(NV, FIT, OUT != 0, false); \
+                           else if (a.w) FWD_AS(NV, FIT, false, OUT != 0); \
+                           else FWD_AS(NV, FIT, false, false); } while (0)
 #define FWD_LONG hipLaunchKernelGGL((iso::rms_forward_long_kernel<T, OUT>), grid, dim3(block), 0, s, a)
         ROWS_NV(nv, fit, FWD, FWD_LONG);
 #undef FWD
+#undef FWD_AS
 #undef FWD_LONG
     }
 }
