@@ -222,9 +222,16 @@ __device__ __forceinline__ float rms_inverse(float ss, double wide, double inv_F
     if (__builtin_expect(wide >= 0.0 || wide != wide, 0)) return (float)(1.0 / __builtin_sqrt(wide * inv_F + (double)eps));
     return __builtin_amdgcn_rsqf(__builtin_fmaf(ss, (float)inv_F, eps));
 }
-// 1 / (sqrt(ss) + eps): v_sqrt_f32 and v_rcp_f32 are within one step
-__device__ __forceinline__ float l2_inverse(float ss, double wide, float eps) {
-    if (__builtin_expect(wide >= 0.0 || wide != wide, 0)) return (float)(1.0 / (__builtin_sqrt(wide) + (double)eps));
+// 1 / (sqrt(ss) + eps): v_sqrt_f32 and v_rcp_f32 are within one step.  `small`: the inverse lies below the normal numbers, whose spacing would cost
+// bits (3e-5 of the value for rows of 33 000 columns near the largest float); it is 2^64 times what it says, for values divided by 2^64.
+__device__ __forceinline__ float l2_inverse(float ss, double wide, float eps, bool& small) {
+    small = false;
+    const bool odd = wide >= 0.0 || wide != wide;
+    if (__builtin_expect(odd || eps > 0x1p100f, 0)) {
+        const double inv = 1.0 / (__builtin_sqrt(odd ? wide : (double)ss) + (double)eps);
+        small = inv < 0x1p-126;
+        return (float)(small ? inv * 0x1p64 : inv);
+    }
     return __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(ss) + eps);
 }
 
@@ -909,8 +916,14 @@ template <class T, int CODE, int NV, int FIT, bool NT> __global__ __launch_bound
     float inv = 1.0f;
     if (a.norm) {
         double wide;
+        bool small;
         const float ss = row_squares(v, row >= 0, tpr, lds, wide);
-        inv = row >= 0 ? l2_inverse(ss, wide, a.eps) : 0.0f;
+        inv = row >= 0 ? l2_inverse(ss, wide, a.eps, small) : 0.0f;
+        if (row >= 0 && small)
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int e = 0; e < N; e++) v[k][e] *= 0x1p-64f;
     }
     if (i >= a.rows) return;
 #pragma unroll
@@ -927,6 +940,7 @@ template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_lo
     const int tpr = a.tpr, t = threadIdx.x;
     const long long i = a.row0 + blockIdx.x, row = read_row(a, i);
     float inv = 1.0f;
+    bool small = false;
     if (a.norm) {
         double ss = 0.0;
         for (int at = t * N; at < a.F; at += tpr * N) {
@@ -936,13 +950,13 @@ template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_lo
             for (int e = 0; e < N; e++) ss += (double)v[e] * (double)v[e];
         }
         ss = row_sum(ss, tpr, lds, 0);
-        inv = row >= 0 ? l2_inverse(0.0f, ss, a.eps) : 0.0f;
+        inv = row >= 0 ? l2_inverse(0.0f, ss, a.eps, small) : 0.0f;
     }
     for (int at = t * N; at < a.F; at += tpr * N) {
         float v[N];
         code_load<CODE, N, TAIL>(a, row, at, v);
 #pragma unroll
-        for (int e = 0; e < N; e++) v[e] *= inv;
+        for (int e = 0; e < N; e++) v[e] = (small ? v[e] * 0x1p-64f : v[e]) * inv;
         row_store<T, N, TAIL>((T*)a.out + i * a.F, at, a.F, v);
     }
 }

@@ -2,7 +2,7 @@
 
 u = 2^-24.  Codes are those of the products rounded to 24 bits (the kernel's own rounding), taken at a smaller exponent.  Scales: top / Q, rstd
 (below the normal numbers here, at least 2^-128 with a half step of 2^-150: 4 u; the sum in 64 bits adds u, the root's float u) and one rounding:
-within the 20 u of ordinary rows."""
+within the 20 u of ordinary rows.  Likewise the normalised read of such a row: the inverse of its length is kept to 24 bits."""
 import pytest
 import torch
 
@@ -72,3 +72,21 @@ def test_a_sum_beyond_the_largest_float_is_an_infinity(code):
     assert bool(torch.isinf(s).all()) and bool(torch.isnan(q.scales).all())
     t = QuantizedRows.from_rows(s, dtype=code)
     assert bool(torch.isnan(t.read()).all())
+
+
+@pytest.mark.parametrize("code", [torch.int8, E4M3])
+@pytest.mark.parametrize("width,group", [(3, None), (64, 32), (129, None), (1024, 128), (4096, None), (20000, None), (36864, 64)])
+def test_normalised_read_of_rows_near_the_largest_float(code, width, group):
+    print(f"case {code} {width} {group}", flush=True)
+    x = make((6, width), F32, 1).clamp(-3, 3) * 1.1e38
+    x[1], x[2] = 3.4e38, x[2] * 1e-30
+    x[3, width // 2:] *= 1e-25                              # groups of ordinary size beside large ones
+    x[4] = 0.0
+    t = QuantizedRows.from_rows(x, dtype=code, group=group)
+    v = t.read().double()
+    for eps in (1e-6, 0.0, 1e38):
+        rows = [0, 1, 2, 3, 5] if eps == 0.0 else list(range(6))             # (a zero row has no direction)
+        want = v / (v.norm(dim=1, keepdim=True) + float(torch.tensor(eps)))
+        for out in (F32, BF16):
+            got = t.read(out_dtype=out, norm_eps=eps)
+            check(got[rows], want[rows], want[rows].abs() * ((2.0 ** -8 if out == BF16 else U) + 20 * U) + 2.0 ** -149, "normalised")
