@@ -554,6 +554,14 @@ class FeatureAdam:
         torch.autograd.graph.increment_version(p)
         self.normalized = (p._version, y, z)
 
+    def release(self):
+        """Let go of the parameter, its gradient, both moments and every table made from it (training is over:
+        ``SegGaussianModel.compact_features``)."""
+        if self.param is not None:
+            self.param.grad = None
+        self.param = self.exp_avg = self.exp_avg_sq = self.normalized = self.leaves = self._pending_yz = None
+        self._zero1 = self._zscale = self._zplace = None
+
     def zero_grad(self, set_to_none: bool = True):
         if set_to_none:
             self.param.grad = None

@@ -123,13 +123,17 @@ class SegGaussianModel:
     def compact_features(self, dtype: torch.dtype = torch.float8_e4m3fn, group: Optional[int] = None) -> QuantizedRows:
         """The trained feature put away in 8 bits: ``_seg_feature`` becomes a ``rows.QuantizedRows`` of the rows the getter returns
         (normalised, eps 1e-6) - a quarter of the bytes - which ``render()`` and ``gather_rows`` read.  For a model that has been
-        trained: the table carries no gradient."""
+        trained: the table carries no gradient, and the model's ``FeatureAdam``, if it has one, lets go of the float table, its gradient and
+        both moments (a ``torch.optim`` optimiser keeps what it holds: :meth:`SegTrainer.compact_features` empties that too).  ``render()``
+        reads the table back into a float32 ``[P,F]`` on every call, which it drops behind it."""
         if isinstance(self._seg_feature, QuantizedRows):
             raise RuntimeError("compact_features: the features are in 8 bits already")
         if self._seg_feature is None:
             raise RuntimeError("compact_features: the model has no features")
         with torch.no_grad():
             table = QuantizedRows.from_rows(row_normalize(self._seg_feature, 1e-6), dtype=dtype, group=group)
+        if getattr(self, "feature_optimizer", None) is not None:
+            self.feature_optimizer.release()
         self._seg_feature, self._seg_cache, self.feature_optimizer = table, None, None
         return table
 
@@ -278,6 +282,23 @@ class SegTrainer:
                 c.sorted_segmap.to(self.device).to(torch.int64).contiguous()
             self.valid_idx[i] = torch.nonzero(c.segmap.reshape(-1) > 0).reshape(-1)
 
+    def compact_features(self, dtype: torch.dtype = torch.float8_e4m3fn, group: Optional[int] = None) -> QuantizedRows:
+        """``SegGaussianModel.compact_features`` for a trainer that is done: the float table, its gradient and the optimiser's moments are
+        let go, whichever optimiser it is, and no further step is taken.  (The buffer of a direct exchange between ranks stays: others
+        have it mapped.)"""
+        table = self.model.compact_features(dtype, group)
+        if not hasattr(self.opt, "release"):
+            for params in self.opt.param_groups:
+                for p in params["params"]:
+                    p.grad = None
+                params["params"] = []
+            self.opt.state.clear()
+        return table
+
+    def _check_trainable(self):
+        if isinstance(self.model._seg_feature, QuantizedRows):
+            raise RuntimeError("SegTrainer: the features were put away in 8 bits (compact_features): there is nothing to train")
+
     def features_in_input_order(self) -> torch.Tensor:
         """The trained ``[P,F]`` feature with rows in the order of the scene passed to the constructor."""
         f = self.model._seg_feature
@@ -306,6 +327,7 @@ class SegTrainer:
         allocator's pools have their steady-state size and the side stream exists — then put parameters, optimiser state and
         the sampling RNG back exactly as they were (so a benchmark's first warm-up step, iteration ``next_it``, is an ordinary
         step)."""
+        self._check_trainable()
         p = self.model._seg_feature
         saved_p = p.detach().clone()
         gen_state = self.gen.get_state()
@@ -370,6 +392,7 @@ class SegTrainer:
         return view_for(it, self.rank, self.world, len(self.cams), seed=self.view_seed)
 
     def step(self, it: int):
+        self._check_trainable()
         if self.high_priority_main and self.device.type == "cuda":
             # the step's own chain on a high-priority stream: the hardware favours its workgroups over those of the side
             # stream (the next view's binning), whose kernels otherwise slow the small loss kernels 2-3x

@@ -1,0 +1,47 @@
+"""Features put away in 8 bits: what training held of them is let go, memory falls by it, and the trainer says that it is done."""
+import gc
+import math
+
+import pytest
+import torch
+
+from instascene_amd.rows import QuantizedRows
+
+pytestmark = pytest.mark.gpu
+
+P, F = 60_000, 32
+
+
+def _trainer(**kw):
+    from instascene_amd import scenes
+    from instascene_amd.harness import SegTrainer
+    sc = scenes.synthetic_scene(P, F, 5, math.log(0.02))
+    return SegTrainer(sc, scenes.ring_cameras(6, 96, 64), device="cuda", sample_batchsize=512, n_labels=8, use_class_feat=True, seed=3, **kw)
+
+
+def _allocated():
+    gc.collect()
+    torch.cuda.synchronize()
+    return torch.cuda.memory_allocated()
+
+
+@pytest.mark.parametrize("kw,by_model", [({}, True), ({}, False), ({"max_grad_norm": 1e-4}, True), ({"fused_update": False, "fused_tail": False}, False)])
+def test_the_float_table_and_the_moments_are_let_go(kw, by_model):
+    from instascene_amd.render import render
+    t = _trainer(**kw)
+    for it in range(3):
+        t.step(it)
+    before = _allocated()
+    table = (t.model if by_model else t).compact_features(torch.int8)
+    freed = before - _allocated()
+    # the parameter and its two moments at least, less the table; allocations are rounded up to 512 bytes, a few small ones aside
+    assert freed >= 3 * 4 * P * F - table.nbytes - (1 << 17), freed
+    for call in (lambda: t.step(3), lambda: t.prime(1)):
+        with pytest.raises(RuntimeError, match="compact_features"):
+            call()
+    with torch.no_grad():
+        out = render(t.cams[0], t.model, t.pipe, t.bg)["seg_feature"]
+    assert out.shape[0] == F and bool(torch.isfinite(out).all())
+    assert t.features_in_input_order().shape == (P, F)
+    assert isinstance(t.model.get_seg_feature, QuantizedRows)
+    t.warm_view_caches()
