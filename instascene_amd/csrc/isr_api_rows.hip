@@ -67,11 +67,12 @@ template <class T, int OUT> void launch_forward(iso::RmsArgs a, hipStream_t s) {
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
         const dim3 grid((unsigned)((n + rpb - 1) / rpb));
+// (so many bytes with one vector per thread do not occur: there are rows enough for two)
 #define FWD_AS(NV, FIT, NT, GAIN) hipLaunchKernelGGL((iso::rms_forward_kernel<T, NV, OUT, FIT, NT, GAIN>), grid, dim3(block), 0, s, a)
-#define FWD(NV, FIT) do { if (OUT == 0) FWD_AS(NV, FIT, false, false); \
-                           else if (nt && a.w) FWD_AS(NV, FIT, OUT != 0, OUT != 0); \
-                           else if (nt) FWD_AS(NV, FIT, OUT != 0, false); \
-                           else if (a.w) FWD_AS(NV, FIT, false, OUT != 0); \
+#define FWD(NV, FIT) do { constexpr bool NT = OUT != 0 && NV > 1, GAIN = OUT != 0; \
+                           if (nt && a.w) FWD_AS(NV, FIT, NT, GAIN); \
+                           else if (nt) FWD_AS(NV, FIT, NT, false); \
+                           else if (a.w) FWD_AS(NV, FIT, false, GAIN); \
                            else FWD_AS(NV, FIT, false, false); } while (0)
 #define FWD_LONG hipLaunchKernelGGL((iso::rms_forward_long_kernel<T, OUT>), grid, dim3(block), 0, s, a)
         ROWS_NV(nv, fit, FWD, FWD_LONG);
@@ -139,7 +140,7 @@ template <class T, int CODE> void launch_read(iso::ReadArgs a, hipStream_t s) {
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += step) {
         const long long n = std::min(step, a.rows - a.row0);
         const dim3 grid((unsigned)((n + rpb - 1) / rpb));
-#define READ(NV, FIT) do { if (nt) hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, FIT, true>), grid, dim3(block), 0, s, a); \
+#define READ(NV, FIT) do { if (nt) hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, FIT, (NV > 1 || FIT != iso::TAIL)>), grid, dim3(block), 0, s, a); \
                             else hipLaunchKernelGGL((iso::rows_read_kernel<T, CODE, NV, FIT, false>), grid, dim3(block), 0, s, a); } while (0)
 #define READ_LONG hipLaunchKernelGGL((iso::rows_read_long_kernel<T, CODE>), grid, dim3(block), 0, s, a)
         ROWS_NV(nv, fit, READ, READ_LONG);
