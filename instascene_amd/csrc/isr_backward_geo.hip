@@ -226,10 +226,8 @@ __global__ __launch_bounds__(64 * NW, 4) void k_render_bwd_geo(
             }
             const bool pre_mine = pre && lane == f_lane;
             if (STATS && pre) st[8]++;
-            // The sums a lane keeps for its splat, as the register PAIRS the packed fp32 instructions take (v_pk_fma_f32 / v_pk_add_f32:
-            // one instruction for two sums, the same IEEE operation per component); the pairing follows the operands that are
-            // already neighbours - (dx, dy), (sx, sy), dL/dp.xy, the even-aligned halves of the pixel's float4s - so that no
-            // register has to be moved to form a pair.
+            // The sums a lane keeps for its splat, two components to a vector; the pairing follows the operands that are
+            // already neighbours - (dx, dy), (sx, sy), dL/dp.xy, the even-aligned halves of the pixel's float4s.
             v2f P01 = {0, 0}, X01 = {0, 0}, Y01 = {0, 0};      // sum dL/dp.xy, sum lx dL/dp.xy, sum ly dL/dp.xy
             v2f XY2 = {0, 0};                                  // (sum lx dL/dp.z, sum ly dL/dp.z)
             v2f PZ2 = {0, 0};                                  // (sum dL/dp.z, sum dL/dz)

@@ -14,7 +14,7 @@
 //   of k.z = fl(fl(px Tw.z) - Tu.z) cancels ~3 decimal digits (px Tw.z ~ Tu.z ~ 1e4, their difference a few pixels times the
 //   depth) and that rounding dominates everything else in rho by two orders of magnitude.  FAST therefore computes k.z and
 //   l.z with EXACTLY those two roundings (bit-identical to EXACT's), the well-conditioned k.xy, l.xy and the cross product
-//   with fused multiply-adds, two components per v_pk_* instruction (8 vector instructions for p), s = p.xy * rcp(p.z), and
+//   with fused multiply-adds (14 vector instructions for p; scalar fp32 throughout, see the Makefile), s = p.xy * rcp(p.z), and
 //   depth = <p, Tw> / p.z = det / p.z with the per-splat det = det[Tu, Tv, Tw]  (<k x l, Tw> = det[k, l, Tw], and adding
 //   multiples of Tw to the other two rows does not change it).  Its rho then follows EXACT's to ~1e-6 relative, so the guard
 //   bands below are narrow.
@@ -118,22 +118,16 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 struct FastRay { float p_x, p_y, p_z, dx, dy, rho2d, rz, sx, sy, rho3d, rho; };
 
 // first half: the intersection and the two squared distances.  pq = the pixel (absolute x, y); operands as the register
-// pairs the packed instructions take them in (a staged record is laid out so that ds_read_b128 delivers exactly these):
+// pairs a staged record keeps them in (laid out so that ds_read_b128 delivers exactly these):
 //   Tuxy = (Tu.x, Tu.y)  Tvxy = (Tv.x, Tv.y)  Twxy = (Tw.x, Tw.y)  Tuvz = (Tu.z, Tv.z)  cxy = the low-pass centre
 __device__ __forceinline__ FastRay fast_ray(v2f pq, v2f Tuxy, v2f Tvxy, v2f Twxy, v2f Tuvz, float Twz, v2f cxy) {
     FastRay r;
     const v2f klz = pq * (v2f){Twz, Twz} - Tuvz;                         // (k.z, l.z): EXACT's two roundings (-ffp-contract=off)
     const v2f kxy = __builtin_elementwise_fma((v2f){pq.x, pq.x}, Twxy, -Tuxy);
     const v2f lxy = __builtin_elementwise_fma((v2f){pq.y, pq.y}, Twxy, -Tvxy);
-    // (p.x, p.y) = l.z (k.y, -k.x) - k.z (l.y, -l.x): two packed instructions whose operand swizzles and signs are instruction
-    // modifiers (the compiler materialises the swapped, half-negated pairs with four extra moves / xors)
-    //   t   = (k.z l.y, -k.z l.x)            src0 = klz.lo twice, src1 = (lxy.hi, -lxy.lo)
-    //   pxy = (l.z k.y - t.lo, -l.z k.x - t.hi)   src0 = klz.hi twice, src1 = (kxy.hi, -kxy.lo), src2 = -t
-    v2f t, pxy;
-    asm("v_pk_mul_f32 %0, %1, %2 op_sel:[0,1] op_sel_hi:[0,0] neg_hi:[0,1]" : "=v"(t) : "v"(klz), "v"(lxy));
-    asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[1,1,0] op_sel_hi:[1,0,1] neg_lo:[0,0,1] neg_hi:[0,1,1]" : "=v"(pxy) : "v"(klz), "v"(kxy), "v"(t));
-    r.p_x = pxy.x;
-    r.p_y = pxy.y;
+    // (p.x, p.y) = l.z (k.y, -k.x) - k.z (l.y, -l.x)
+    r.p_x = __builtin_fmaf(klz.y, kxy.y, -(klz.x * lxy.y));
+    r.p_y = __builtin_fmaf(klz.y, -kxy.x, klz.x * lxy.x);
     r.p_z = __builtin_fmaf(kxy.x, lxy.y, -(kxy.y * lxy.x));
     const v2f d = cxy - pq;
     r.dx = d.x;
@@ -141,15 +135,14 @@ __device__ __forceinline__ FastRay fast_ray(v2f pq, v2f Tuxy, v2f Tvxy, v2f Twxy
     const float hh = __builtin_fmaf(r.dy, r.dy, r.dx * r.dx);
     r.rho2d = hh + hh;                                  // FilterInvSquare = 2
     r.rz = __builtin_amdgcn_rcpf(r.p_z);
-    const v2f sxy = pxy * (v2f){r.rz, r.rz};
-    r.sx = sxy.x;
-    r.sy = sxy.y;
+    r.sx = r.p_x * r.rz;
+    r.sy = r.p_y * r.rz;
     r.rho3d = __builtin_fmaf(r.sy, r.sy, r.sx * r.sx);
     r.rho = fminf(r.rho3d, r.rho2d);
     return r;
 }
 // The same split by pixel column and row, for a kernel that walks the pixels of a block for one splat per lane (k depends on
-// the column only, l on the row only): bit-identical to fast_ray (the packed instructions round each half like the scalar ones).
+// the column only, l on the row only): bit-identical to fast_ray (the same operations on the same values).
 struct FastHalf { v2f xy; float z; };
 __device__ __forceinline__ FastHalf fast_k(float pxf, const F3 Tu, const F3 Tw) {
     return {__builtin_elementwise_fma((v2f){pxf, pxf}, (v2f){Tw.x, Tw.y}, -(v2f){Tu.x, Tu.y}), pxf * Tw.z - Tu.z};
@@ -160,20 +153,16 @@ __device__ __forceinline__ FastHalf fast_l(float pyf, const F3 Tv, const F3 Tw) 
 __device__ __forceinline__ FastRay fast_ray_kl(const FastHalf& k, const FastHalf& l, float dx, float dy) {
     FastRay r;
     const v2f klz = {k.z, l.z};
-    v2f t, pxy;
-    asm("v_pk_mul_f32 %0, %1, %2 op_sel:[0,1] op_sel_hi:[0,0] neg_hi:[0,1]" : "=v"(t) : "v"(klz), "v"(l.xy));
-    asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[1,1,0] op_sel_hi:[1,0,1] neg_lo:[0,0,1] neg_hi:[0,1,1]" : "=v"(pxy) : "v"(klz), "v"(k.xy), "v"(t));
-    r.p_x = pxy.x;
-    r.p_y = pxy.y;
+    r.p_x = __builtin_fmaf(klz.y, k.xy.y, -(klz.x * l.xy.y));
+    r.p_y = __builtin_fmaf(klz.y, -k.xy.x, klz.x * l.xy.x);
     r.p_z = __builtin_fmaf(k.xy.x, l.xy.y, -(k.xy.y * l.xy.x));
     r.dx = dx;
     r.dy = dy;
     const float hh = __builtin_fmaf(r.dy, r.dy, r.dx * r.dx);
     r.rho2d = hh + hh;
     r.rz = __builtin_amdgcn_rcpf(r.p_z);
-    const v2f sxy = pxy * (v2f){r.rz, r.rz};
-    r.sx = sxy.x;
-    r.sy = sxy.y;
+    r.sx = r.p_x * r.rz;
+    r.sy = r.p_y * r.rz;
     r.rho3d = __builtin_fmaf(r.sy, r.sy, r.sx * r.sx);
     r.rho = fminf(r.rho3d, r.rho2d);
     return r;

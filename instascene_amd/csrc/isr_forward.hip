@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256, 4) void k_render_fwd(
     float C0 = 0, C1 = 0, C2 = 0, N0 = 0, N1 = 0, N2 = 0, D = 0, M1 = 0, M2 = 0, distortion = 0, median_depth = 0;
     // FAST arithmetic, 32-channel chunk: the feature accumulation  E[pix][ch] += w(pix, splat) * feat[splat][ch]  runs on
     // the matrix cores, two contributing splats per v_mfma_f32_32x32x2_f32 pair (one for pixels 0..31 of the wave, one
-    // for 32..63) — 16 packed FMAs + 8 LDS reads per splat leave the VALU, which is what bounds this kernel.
+    // for 32..63) — 32 FMAs + 8 LDS reads per splat leave the VALU, which is what bounds this kernel.
     constexpr bool MF = Math::fast && FCH == 32;
     float E[(FCH > 0 && !MF) ? FCH : 1];
 #pragma unroll

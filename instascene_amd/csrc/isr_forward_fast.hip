@@ -24,7 +24,7 @@ namespace isr {
 
 constexpr int FF_BATCH = 128;       // instances staged per round
 constexpr int FF_RS = 24;           // staged floats per instance (six float4)
-// staged record (the pairs fast_ray's packed instructions take, each an aligned register pair of a ds_read_b128):
+// staged record (the pairs fast_ray takes, each an aligned register pair of a ds_read_b128):
 //                 q0 = Tu.x, Tu.y, Tv.x, Tv.y
 //                 q1 = Tw.x, Tw.y, Tu.z, Tv.z
 //                 q2 = Tw.z, band.hi, cx, cy      alpha < 1/255 is certain for rho > band.hi

@@ -5,10 +5,10 @@
 set -e
 cd "$(dirname "$0")/../instascene_amd/csrc"
 name=$1; unit=$2; shift 2
-make -s -j5
+make -s -j6
 obj=../../build/csrc
 mkdir -p $obj/var_$name
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math -Wall -Wno-unused-function "$@" -c $unit.hip -o $obj/var_$name/$unit.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c $unit.hip -o $obj/var_$name/$unit.o
 others=$(ls $obj/*.o | grep -v "/$unit.o")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -fPIC -shared $others $obj/var_$name/$unit.o -o ../libinstascene_hip_$name.so
 echo ../libinstascene_hip_$name.so
