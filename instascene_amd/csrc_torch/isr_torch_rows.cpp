@@ -94,7 +94,6 @@ struct Rows {
     Rows() = default;
     explicit Rows(const Tensor& x) { if (x.defined()) t = rows2d(x); }
     const void* data() const { return t.defined() ? t.data_ptr() : nullptr; }
-    void* data_w() const { return t.defined() ? t.data_ptr() : nullptr; }
     long long stride() const { return t.defined() ? t.stride(0) : 0; }
 };
 const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }

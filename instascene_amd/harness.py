@@ -168,7 +168,8 @@ class SegTrainer:
                  multiview=False, seed=0, rank=0, world=1, prefetch_geometry=None, fused_update=None, sampled_path=True,
                  fused_tail=None, batched_losses=None, spatial_sort=True, fused_sampling=None, max_grad_norm=None):
         """``max_grad_norm``: clip the (summed) gradient of ``_seg_feature`` to this 2-norm in every step; the norm of the last one is in
-        ``last_grad_norm`` (a scalar on the device)."""
+        ``last_grad_norm`` (a scalar on the device).  The norm has to be known before the first row is stepped: the gradient is written out and
+        read again, and the step leaves the one-entry tail (1.68 -> 1.85 ms at 1.5 M Gaussians, 32 channels, 1080p)."""
         self.device = torch.device(device)
         self.max_grad_norm = None if max_grad_norm is None else check_max_norm("SegTrainer", max_grad_norm)
         # Gaussians stored in Z-order of their centres (once, here): neighbours in memory are neighbours on screen, which
@@ -1039,7 +1040,7 @@ class RgbTrainer:
     def __init__(self, scene, cameras, targets, device="cuda", lambda_dssim=0.2, lambda_normal=0.05, lambda_dist=0.0,
                  rank=0, world=1, densify=None, scene_extent=None, spatial_sort=True, fused_update=None, max_grad_norm=None):
         """``max_grad_norm``: clip the gradients of the six parameter groups together to this 2-norm in every step; the norm of the last one
-        is in ``last_grad_norm``.  ``spatial_sort``: store the Gaussians in Z-order of their centres (a row permutation, once, here; rows that the
+        is in ``last_grad_norm`` (the step leaves the one-entry tail: 0.736 -> 0.746 ms at 300 k Gaussians).  ``spatial_sort``: store the Gaussians in Z-order of their centres (a row permutation, once, here; rows that the
         density control appends later go to the end).  ``densify``: None (off) or a dict overriding the reference's schedule (arguments/__init__.py:106-125):
         ``from_iter=500, until_iter=15000, interval=100, opacity_reset_interval=3000, grad_threshold=0.0002,
         opacity_cull=0.05, percent_dense=0.01``; ``scene_extent`` = the reference's ``cameras_extent``."""

@@ -33,7 +33,8 @@ def _ext():
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
     """``y = s / sqrt(mean(s^2) + eps) * weight`` over the last dimension, ``s = x + residual``; returns ``y``, or ``(y, s)`` with a
     residual.  float32, bfloat16 or float16, rows of any width and stride; everything between input and output is held in 32 bits
-    (the sum of squares in 64), ``y`` and ``s`` are rounded once.  ``weight`` is float32 or of x's type.  Differentiable in ``x``,
+    (the sum of squares too, formed again in 64 where it leaves [1e-30, 1e37] and always for rows beyond the registers), ``y`` and ``s`` are
+    rounded once.  ``weight`` is float32 or of x's type.  Differentiable in ``x``,
     ``weight`` and ``residual``."""
     y, s = _ext().rms_norm(x, weight, eps, residual)
     return y if s is None else (y, s)
