@@ -222,17 +222,24 @@ __device__ __forceinline__ float rms_inverse(float ss, double wide, double inv_F
     if (__builtin_expect(wide >= 0.0 || wide != wide, 0)) return (float)(1.0 / __builtin_sqrt(wide * inv_F + (double)eps));
     return __builtin_amdgcn_rsqf(__builtin_fmaf(ss, (float)inv_F, eps));
 }
-// 1 / (sqrt(ss) + eps): v_sqrt_f32 and v_rcp_f32 are within one step.  `small`: the inverse lies below the normal numbers, whose spacing would cost
-// bits (3e-5 of the value for rows of 33 000 columns near the largest float); it is 2^64 times what it says, for values divided by 2^64.
-__device__ __forceinline__ float l2_inverse(float ss, double wide, float eps, bool& small) {
-    small = false;
+// A row's values over its length + eps: v inv, corrected once by its exact remainder v - q d (as a division rounds; the product alone is a step
+// further off).  `small`: the inverse lies below the normal numbers, whose spacing would cost bits (3e-5 of the value for rows of 33 000 columns
+// near the largest float); d is then 2^64 times smaller than it is, for values divided by 2^64.
+struct Length { float d, inv; bool small; };
+__device__ __forceinline__ Length l2_length(float ss, double wide, float eps) {
     const bool odd = wide >= 0.0 || wide != wide;
     if (__builtin_expect(odd || eps > 0x1p100f, 0)) {
-        const double inv = 1.0 / (__builtin_sqrt(odd ? wide : (double)ss) + (double)eps);
-        small = inv < 0x1p-126;
-        return (float)(small ? inv * 0x1p64 : inv);
+        const double d = __builtin_sqrt(odd ? wide : (double)ss) + (double)eps;
+        const bool small = d > 0x1p126;
+        const double e = small ? d * 0x1p-64 : d;
+        return {(float)e, e > 0.0 && e < 0x1p-126 ? 0.0f : (float)(1.0 / e), small};           // (so short: a row of zeros, and an eps below the normal numbers)
     }
-    return __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(ss) + eps);
+    const float d = __builtin_sqrtf(ss) + eps;
+    return {d, 1.0f / d, false};
+}
+__device__ __forceinline__ float over_length(float v, const Length& l) {
+    const float q = v * l.inv;
+    return __builtin_fmaf(__builtin_fmaf(-q, l.d, v), l.inv, q);
 }
 
 // ---- 8-bit codes -----------------------------------------------------------------------------------------------------------------
@@ -913,24 +920,24 @@ template <class T, int CODE, int NV, int FIT, bool NT> __global__ __launch_bound
     float v[NV][N];
 #pragma unroll
     for (int k = 0; k < NV; k++) code_load<CODE, N, FIT>(a, row, (t + k * tpr) * N, v[k]);
-    float inv = 1.0f;
     if (a.norm) {
         double wide;
-        bool small;
         const float ss = row_squares(v, row >= 0, tpr, lds, wide);
-        inv = row >= 0 ? l2_inverse(ss, wide, a.eps, small) : 0.0f;
-        if (row >= 0 && small)
+        const Length l = row >= 0 ? l2_length(ss, wide, a.eps) : Length{0.0f, 0.0f, false};
+        if (l.small)
 #pragma unroll
             for (int k = 0; k < NV; k++)
 #pragma unroll
                 for (int e = 0; e < N; e++) v[k][e] *= 0x1p-64f;
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int e = 0; e < N; e++) v[k][e] = over_length(v[k][e], l);
     }
     if (i >= a.rows) return;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int at = (t + k * tpr) * N;
-#pragma unroll
-        for (int e = 0; e < N; e++) v[k][e] *= inv;
         if (at < a.F) row_store<T, N, FIT, NT>((T*)a.out + i * a.F, at, a.F, v[k]);
     }
 }
@@ -939,8 +946,7 @@ template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_lo
     __shared__ double lds[2][16];
     const int tpr = a.tpr, t = threadIdx.x;
     const long long i = a.row0 + blockIdx.x, row = read_row(a, i);
-    float inv = 1.0f;
-    bool small = false;
+    Length l = {1.0f, 1.0f, false};
     if (a.norm) {
         double ss = 0.0;
         for (int at = t * N; at < a.F; at += tpr * N) {
@@ -950,13 +956,13 @@ template <class T, int CODE> __global__ __launch_bounds__(512) void rows_read_lo
             for (int e = 0; e < N; e++) ss += (double)v[e] * (double)v[e];
         }
         ss = row_sum(ss, tpr, lds, 0);
-        inv = row >= 0 ? l2_inverse(0.0f, ss, a.eps, small) : 0.0f;
+        l = row >= 0 ? l2_length(0.0f, ss, a.eps) : Length{0.0f, 0.0f, false};
     }
     for (int at = t * N; at < a.F; at += tpr * N) {
         float v[N];
         code_load<CODE, N, TAIL>(a, row, at, v);
 #pragma unroll
-        for (int e = 0; e < N; e++) v[e] = (small ? v[e] * 0x1p-64f : v[e]) * inv;
+        for (int e = 0; e < N; e++) v[e] = over_length(l.small ? v[e] * 0x1p-64f : v[e], l);
         row_store<T, N, TAIL>((T*)a.out + i * a.F, at, a.F, v);
     }
 }

@@ -90,3 +90,5 @@ def test_normalised_read_of_rows_near_the_largest_float(code, width, group):
         for out in (F32, BF16):
             got = t.read(out_dtype=out, norm_eps=eps)
             check(got[rows], want[rows], want[rows].abs() * ((2.0 ** -8 if out == BF16 else U) + 20 * U) + 2.0 ** -149, "normalised")
+    zeros = t.read(slice(4, 5), norm_eps=1e-40)              # (an eps below the normal numbers)
+    assert bool((zeros == 0).all()) and bool(torch.isnan(t.read(slice(4, 5), norm_eps=0.0)).all())
