@@ -47,8 +47,9 @@ SIMDS, CLOCK_GHZ = 1024, 2.4      # MI355X: 256 CUs x 4 SIMDs
 # (v_pk_fma_f32), SGPR-writing compares, v_cndmask with an SGPR mask, DPP, v_readlane: 500-570 G/s (x1.5); v_rcp / v_exp /
 # v_permlane32_swap: 290-300 G/s (x2.9); ds_read_b128: 150 G/s for any address pattern (4 cycles per CU).
 ISSUE_PEAK_PLAIN_G = 850.0
-# the blend kernel's walk, counted by class in its ISA: ~77 plain-equivalent issue slots for 66 vector instructions
-ISSUE_MIX_WEIGHT = 77.0 / 66.0
+# the blend kernel's walk, counted by class in its ISA: ~82 plain-equivalent issue slots for 75 vector instructions (scalar fp32: 66 with nine
+# packed ones were 77 slots)
+ISSUE_MIX_WEIGHT = 82.0 / 75.0
 
 
 def csrc_tree_hash():
