@@ -83,11 +83,13 @@ int check_code(const char* what, at::ScalarType t) {
     TORCH_CHECK_TYPE(code_type(t) != 0, what, ": dtype must be torch.int8 or torch.float8_e4m3fn, not ", t);
     return code_type(t);
 }
-// [rows, F] with the columns of a row next to each other (a copy only where they are not)
+// [rows, F] with the columns of a row next to each other (a copy only where they are not, or where the memory holds the negative of the values)
+Tensor as_stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 Tensor rows2d(const Tensor& t) {
     Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)});
-    return r.size(1) == 1 || r.stride(1) == 1 ? r : r.contiguous();
+    return as_stored(r.size(1) == 1 || r.stride(1) == 1 ? r : r.contiguous());
 }
+Tensor gain_of(const Tensor& w) { return w.defined() ? as_stored(w.contiguous()) : Tensor(); }
 // a tensor that may be absent, as rows
 struct Rows {
     Tensor t;
@@ -102,7 +104,7 @@ struct Forward { Tensor y, s, rstd; };
 Forward norm_forward(const Tensor& x, const Tensor& weight, double eps, const Tensor& residual, bool want_rstd) {
     const c10::DeviceGuard guard(x.device());
     const Rows x2(x), r2(residual);
-    const Tensor w = weight.defined() ? weight.contiguous() : Tensor();
+    const Tensor w = gain_of(weight);
     Forward f;
     f.y = at::empty(x.sizes(), x.options());
     if (residual.defined()) f.s = at::empty(x.sizes(), x.options());
@@ -162,7 +164,7 @@ private:
         const Rows x2(x), r2(residual), g2(gy), q2(gs);
         const int type = row_type(x.scalar_type());
         const int64_t n = x2.t.size(0), F = x2.t.size(1);
-        const Tensor w = weight.defined() ? weight.contiguous() : Tensor();
+        const Tensor w = gain_of(weight);
         Tensor ds, dw, scratch;
         if (need_x || need_r) ds = at::empty(x.sizes(), x.options());
         size_t bytes = 0;
@@ -207,7 +209,7 @@ std::tuple<Tensor, Tensor, OptTensor> rms_norm_quantized(const Tensor& x, const 
     const c10::DeviceGuard guard(x.device());
     const int64_t n = x.size(0), F = x.size(1), G = check_group(what, F, group);
     const Rows x2(x), r2(residual_.value_or(Tensor()));
-    const Tensor w = weight_ ? weight_->contiguous() : Tensor();
+    const Tensor w = gain_of(weight_.value_or(Tensor()));
     Tensor codes = at::empty({n, F}, x.options().dtype(dtype)), scales = at::empty({n, F / G}, x.options().dtype(at::kFloat)), s;
     if (residual_) s = at::empty({n, F}, x.options());
     check(iso_rms_norm_quant(row_type(x.scalar_type()), code, n, (int)F, (int)G, x2.data(), x2.stride(), r2.data(), r2.stride(), ptr(w),

@@ -49,3 +49,20 @@ def test_inference_mode():
     assert torch.equal(y, rms_norm(x.clone(), w.detach(), residual=x.clone())[0])
     assert torch.equal(got, QuantizedRows.from_rows(y[1:2].clone()).read())
     assert q.codes.shape == (300, 64)
+
+
+def test_views_that_negate_their_memory():
+    """The imaginary part of a conjugate is a view whose memory holds the negative of its values (here one column wide, and as torch makes
+    such a view of any tensor)."""
+    c = torch.view_as_complex(make((50, 1, 2), F32, 1))
+    x = torch.imag(torch.conj(c))
+    assert x.is_neg() and torch.equal(x, -c.imag)
+    assert torch.equal(rms_norm(x), rms_norm(x.clone())) and torch.equal(QuantizedRows.from_rows(x).read(), QuantizedRows.from_rows(x.clone()).read())
+    x, r, w, gy = (torch._neg_view(t) for t in (make((9, 40), F32, 2), make((9, 40), F32, 3), make((40,), F32, 4), make((9, 40), F32, 5)))
+    for a, b in zip(rms_norm(x, w, residual=r), rms_norm(x.clone(), w.clone(), residual=r.clone())):
+        assert torch.equal(a, b)
+    a, b = (rms_norm_quantized(t[0], t[1], dtype=torch.int8) for t in ((x, w), (x.clone(), w.clone())))
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    leaf, gain = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    for one, other in zip(torch.autograd.grad(rms_norm(leaf, gain), (leaf, gain), gy), torch.autograd.grad(rms_norm(leaf, gain), (leaf, gain), gy.clone())):
+        assert torch.equal(one, other)
